@@ -447,6 +447,19 @@ class Buffer:
         return self._like(self._dispatch(CustomOps.CACHED_ATTENTION, q=self, k_store=k_store, v_store=v_store, n=n,
                                          n_head=n_head, scale=scale, hidden=hidden))
 
+    @staticmethod
+    def rotary(parts: list, **kw) -> list:
+        """parts: one or two (Buffer, heads, pitch) on one device, turned by rotary positions in one launch; the results are shaped
+        like them where rows are `heads * d` apart."""
+        outs = dispatcher.dispatch(op=CustomOps.ROTARY, device=parts[0][0].device, parts=parts, **kw)
+        return [x if kw.get("inplace") else x._like(p) for (x, _, _), p in zip(parts, outs)]
+
+    def adjust_logits(self, history: "Buffer | None", lengths: "Buffer | None", penalties: tuple, bias: "Buffer | None",
+                      hidden: "Buffer | None") -> "Buffer":
+        """self: (B, V) logits; penalties for the tokens of the history, a bias and a mask, as nn.adjust_logits describes them."""
+        return self._like(self._dispatch(CustomOps.ADJUST_LOGITS, logits=self, history=history, lengths=lengths, penalties=penalties,
+                                         bias=bias, hidden=hidden))
+
     def log_softmax(self, dim: int) -> "Buffer":
         return self._unary(CustomOps.LOG_SOFTMAX, dim=dim)
 

@@ -100,6 +100,11 @@ class CustomOps(_Op):
     DECODE_EMBED = auto()           # the input of a decoding step (token + position embedding, cache-row mask) from device-resident state
     DECODE_NEXT = auto()            # argmax of the logits, appended to the token buffer, made the next token; the index advanced
     DECODE_SAMPLE = auto()          # the same with the token drawn from softmax(logits / temperature) by a given uniform number
+    ROTARY = auto()                 # rotary positions of one or two (rows, heads * d) tensors, one kernel; its own transpose with the angles reversed
+    CACHE8_WRITE = auto()           # new keys and values into the 8-bit cache: blocks of 64 tokens and a head quantised as they fill up
+    CACHE8_ATTEND = auto()          # attention of new positions over the 8-bit cache
+    CACHE8_READ = auto()            # the values that the 8-bit cache stands for
+    ADJUST_LOGITS = auto()          # penalties for tokens said before, a bias and a mask on logits, one kernel
     RMSNORM = auto()                # (x * rsqrt(mean(x^2) + eps)) * w over the last axis, one kernel
     RMSNORM_BWD = auto()            # its backward: dx in one kernel, dw by partial rows + a column sum
 

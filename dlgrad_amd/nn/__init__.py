@@ -8,6 +8,7 @@ from dlgrad_amd.device import Device
 from dlgrad_amd.nn import optim, utils  # noqa: F401
 from dlgrad_amd.tensor import Tensor
 from dlgrad_amd.nn import datasets  # noqa: E402,F401  (uses Tensor)
+from dlgrad_amd.nn.lm import QuantizedKVCache, Rotary, adjust_logits, rotary_frequencies  # noqa: E402,F401
 
 
 class Linear:

@@ -684,6 +684,18 @@ class SelfAttentionQKV(OP):
         return self._grads(upstream_grad, plus), ((0,) if plus is not None else ())
 
 
+class Rotary(OP):
+    """A tensor turned by rotary positions (nn.Rotary), which the caller has computed: queries and keys turn in one launch and are
+    one node each.  The map is linear; backward is its transpose, the same kernel with the angles reversed."""
+
+    def forward(self, x: Buffer, turned: Buffer, rope, n_head: int, geometry: tuple, positions: Buffer | None, start: Buffer | None, back: bool) -> Buffer:
+        self.rope, self.how = rope, (n_head, geometry, positions, start, back)
+        return turned
+
+    def backward(self, upstream_grad: Buffer) -> tuple:
+        return (self.rope.turn_back(upstream_grad, *self.how),)
+
+
 def use_fused_rmsnorm(x, weight) -> bool:
     if not (FUSED and x.device is Device.HIP):
         return False

@@ -451,8 +451,8 @@ class Buffer:
     def rotary(parts: list, **kw) -> list:
         """parts: one or two (Buffer, heads, pitch) on one device, turned by rotary positions in one launch; the results are shaped
         like them where rows are `heads * d` apart."""
-        outs = dispatcher.dispatch(op=CustomOps.ROTARY, device=parts[0][0].device, parts=parts, **kw)
-        return [x if kw.get("inplace") else x._like(p) for (x, _, _), p in zip(parts, outs)]
+        outs = _dispatch_table[(CustomOps.ROTARY, parts[0][0].device)](parts=parts, **kw)
+        return [p[0] for p in parts] if kw.get("inplace") else [p[0]._like(o) for p, o in zip(parts, outs)]
 
     def adjust_logits(self, history: "Buffer | None", lengths: "Buffer | None", penalties: tuple, bias: "Buffer | None",
                       hidden: "Buffer | None") -> "Buffer":

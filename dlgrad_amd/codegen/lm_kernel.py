@@ -135,8 +135,11 @@ extern "C" __global__ __launch_bounds__(256) void {name}(const float* x0, float*
 # logits
 # =====================================================================================
 
+LOGITS_PACKED_L = 65535      # the longest history whose counts fit 16 bits
+
+
 @cache
-def adjust_logits_kernel(items: int, vec: bool) -> tuple[str, str, str]:
+def adjust_logits_kernel(items: int, vec: bool, packed: bool) -> tuple[str, str, str]:
     """y = logits (B, V) with what has been said already made less likely, a bias added and forbidden tokens removed:
     for a token that occurs c > 0 times among the first lengths[b] entries of history[b],
       x = x / repetition if x > 0 else x * repetition, then x - (presence + frequency * c);
@@ -146,9 +149,11 @@ def adjust_logits_kernel(items: int, vec: bool) -> tuple[str, str, str]:
     A block owns 256 * items consecutive tokens of one row and counts only those: their counters lie in LDS, every
     block walks the whole history of its row (which stays in L2: 4 bytes an entry) and bumps the counters of its own
     tokens with integer atomics, whose order does not matter.  So there is one launch, no count array in memory and
-    no sort.  The logits are loaded before the walk and used after it.  vec: 16-byte accesses (V % 4 == 0)."""
+    no sort.  packed: two 16-bit counters to a word, for histories of at most 65535 -- half the LDS, twice the blocks on a
+    compute unit.  The first 16 entries a thread walks and its logits are loaded before the counters are cleared, so all of
+    these reads are on their way together.  vec: 16-byte accesses (V % 4 == 0)."""
     assert items in (4, 8, 16, 32)
-    name = f"adjust_logits_i{items}_{'v4' if vec else 'v1'}"
+    name = f"adjust_logits_i{items}_{'v4' if vec else 'v1'}{'_h' if packed else ''}"
     W = 4 if vec else 1
     NV = items // W
     if vec:
@@ -160,6 +165,14 @@ def adjust_logits_kernel(items: int, vec: bool) -> tuple[str, str, str]:
     else:
         load, bload = "x[k][0] = lrow[v];", "x[k][0] += brow[v];"
         hload, store = "if (hrow[v] > 0.0f) x[k][0] = NINF;", "yrow[v] = x[k][0];"
+    words = 128 * items if packed else 256 * items
+    bump = "atomicAdd(&count[at >> 1], 1u << (16u * (at & 1u)))" if packed else "atomicAdd(&count[at], 1u)"
+    if vec:
+        counts = ("const uint2 c2 = *reinterpret_cast<const uint2*>(&count[at >> 1]); const u32 c[4] = {c2.x & 0xffffu, c2.x >> 16, c2.y & 0xffffu, c2.y >> 16};"
+                  if packed else "const uint4 c4 = *reinterpret_cast<const uint4*>(&count[at]); const u32 c[4] = {c4.x, c4.y, c4.z, c4.w};")
+    else:
+        counts = "const u32 c[1] = {(count[at >> 1] >> (16u * (at & 1u))) & 0xffffu};" if packed else "const u32 c[1] = {count[at]};"
+    any_of = " | ".join(f"c[{i}]" for i in range(W))
     src = f"""{PRELUDE}
 #define NINF (-__builtin_inff())
 #define SLICE {256 * items}u
@@ -167,42 +180,48 @@ extern "C" __global__ __launch_bounds__(256) void {name}(const float* __restrict
         const float* __restrict__ lengths, const float* __restrict__ bias, const float* __restrict__ hidden, float* __restrict__ y,
         const float* __restrict__ rep_p, const float* __restrict__ pre_p, const float* __restrict__ fre_p,
         u32 V, u32 L, u32 bias_step, u32 hidden_step, float rep, float pre, float fre) {{
-    __shared__ u32 count[SLICE];
+    __shared__ __attribute__((aligned(16))) u32 count[{words}];
     const u32 t = threadIdx.x, v0 = blockIdx.x * SLICE;
     const u64 b = blockIdx.y;
     const float* __restrict__ lrow = logits + b * V;
     float* __restrict__ yrow = y + b * V;
+    const float* __restrict__ said = history + b * L;
+    float first[16];
+    #pragma unroll
+    for (u32 k = 0; k < 16u; ++k) {{ const u32 i = k * 256u + t; first[k] = i < L ? said[i] : -1.0f; }}
+    const float ln = (L && lengths) ? lengths[b] : (float)L;
+    const u32 n = ln >= (float)L ? L : ln > 0.0f ? (u32)ln : 0u;             // (a NaN counts nothing)
     float x[{NV}][{W}];
     #pragma unroll
     for (u32 k = 0; k < {NV}u; ++k) {{
         const u32 v = v0 + (k * 256u + t) * {W}u;
         if (v < V) {{ {load} }}
     }}
-    u32 n = 0u;
     if (L) {{
-        const float ln = lengths ? lengths[b] : (float)L;
-        n = ln >= (float)L ? L : ln > 0.0f ? (u32)ln : 0u;                   // (a NaN counts nothing)
-        for (u32 k = t; k < SLICE; k += 256u) count[k] = 0u;
+        for (u32 k = t; k < {words}u; k += 256u) count[k] = 0u;
         __syncthreads();
-        const float* __restrict__ said = history + b * L;
-        #pragma unroll 4
-        for (u32 k = t; k < n; k += 256u) {{
-            const float id = said[k];
+        auto bump = [&](float id) {{
             if (id >= (float)v0 && id < 4294967040.0f) {{
                 const u32 at = (u32)id - v0;
-                if (at < SLICE) atomicAdd(&count[at], 1u);
+                if (at < SLICE) {bump};
             }}
-        }}
+        }};
+        #pragma unroll
+        for (u32 k = 0; k < 16u; ++k) if (k * 256u + t < n) bump(first[k]);
+        #pragma unroll 8
+        for (u32 k = 4096u + t; k < n; k += 256u) bump(said[k]);
         __syncthreads();
     }}
     if (n) {{
         const float r = rep_p ? rep_p[b] : rep, p = pre_p ? pre_p[b] : pre, f = fre_p ? fre_p[b] : fre;
         #pragma unroll
         for (u32 k = 0; k < {NV}u; ++k) {{
-            #pragma unroll
-            for (u32 i = 0; i < {W}u; ++i) {{
-                const u32 c = count[(k * 256u + t) * {W}u + i];
-                if (c) x[k][i] = (x[k][i] > 0.0f ? x[k][i] / r : x[k][i] * r) - (p + f * (float)c);
+            const u32 at = (k * 256u + t) * {W}u;
+            {counts}
+            if ({any_of}) {{
+                #pragma unroll
+                for (u32 i = 0; i < {W}u; ++i)
+                    if (c[i]) x[k][i] = (x[k][i] > 0.0f ? x[k][i] / r : x[k][i] * r) - (p + f * (float)c[i]);
             }}
         }}
     }}
@@ -249,7 +268,7 @@ static __device__ __forceinline__ void cache8_extent(const float* __restrict__ l
 
 
 @cache
-def cache8_write_kernel(DP: int, vec: bool) -> tuple[str, str, str]:
+def cache8_write_kernel(DP: int, vec: bool, NT: int = 1024) -> tuple[str, str, str]:
     """New key and value rows k, v (B, T, H * d) into the 8-bit cache of one layer, at positions lengths[b] .. of each sequence
     (the first counts[b] rows of each, all T without counts; rows that the cache has no room for are dropped).
 
@@ -258,36 +277,69 @@ def cache8_write_kernel(DP: int, vec: bool) -> tuple[str, str, str]:
     the cache holds depends on the tokens alone and not on the calls that brought them.  Key codes lie as [64][DP] bytes, value
     codes transposed, [DP][64], each code + 128; two tails of 64 rows per head, block i's in tail i & 1.
 
-    The quotient is rounded exactly: q = rint(x * (1 / scale)) may be off by one next to a half, and x - q * scale is
-    representable (both are multiples of the unit of the smaller one, and it is below two scales), so one fused
-    multiply-add gives it without error and the comparison with half a scale decides.
+    The quotient is rounded exactly: q = rint(x * (1 / scale)) may be off by one next to a half.  There x - q * scale, which is
+    representable (both are multiples of the unit of the smaller one, and it is below two scales), comes without error from
+    one fused multiply-add, and the comparison with half a scale decides.
 
     A row that holds a NaN or an infinity is kept as NaN in the tail, and a block with such a row gets NaN for its scales:
     every output that sees it is NaN, and the codes stay whole numbers.
 
-    One workgroup of 256 threads per (block of 64, head, sequence); a thread holds 4 tokens by 4 columns of keys and values
-    at a time.  Workgroup 0 of a head completes the block that the call starts in and then stores the rows of the block it
-    ends in, in this order, because both may use the same tail.  Bound by memory: 4 bytes read and 1 written per element."""
-    name = f"cache8_write_d{DP}_{'v4' if vec else 'v1'}"
-    IT = (DP + 63) // 64                     # items of 4 tokens by 4 columns per thread
-    ld = ("const float4 f = *reinterpret_cast<const float4*>(src + c0);" if vec else
-          "const float4 f = make_float4(c0 < d ? src[c0] : 0.0f, c0 + 1u < d ? src[c0 + 1u] : 0.0f, c0 + 2u < d ? src[c0 + 2u] : 0.0f, c0 + 3u < d ? src[c0 + 3u] : 0.0f);")
+    One workgroup of NT threads per (block of 64, head, sequence), a thread per four columns of a row (16 DP / NT times).  Workgroup 0 of a head completes the block that the call starts in and then stores
+    the rows of the block it ends in, in this order, because both may use the same tail.  Bound by memory for long calls: 4 bytes
+    read and 1 written per element."""
+    name = f"cache8_write_d{DP}_{'v4' if vec else 'v1'}_t{NT}"
+    IT = -(-16 * DP // NT)                     # four columns of a row per thread, so many times
+    if vec:
+        # one load whatever the row is: a choice between two loads would wait for one before the other
+        load = """const float* pk = row < lo || c0 >= d ? tk + row * DP + c0 : kh + at * kp + c0;
+            const float* pv = row < lo || c0 >= d ? tv + row * DP + c0 : vh + at * vp + c0;
+            fk = *reinterpret_cast<const float4*>(there ? pk : tk);
+            fv = *reinterpret_cast<const float4*>(there ? pv : tv);
+            if (!there || (row >= lo && c0 >= d)) { fk = make_float4(0.f, 0.f, 0.f, 0.f); fv = fk; }"""
+    else:
+        load = """if (there && row < lo) { fk = *reinterpret_cast<const float4*>(tk + row * DP + c0); fv = *reinterpret_cast<const float4*>(tv + row * DP + c0); }
+            else if (there) {
+                const float* pk = kh + at * kp;
+                const float* pv = vh + at * vp;
+                if (c0 < d) { fk.x = pk[c0]; fv.x = pv[c0]; }
+                if (c0 + 1u < d) { fk.y = pk[c0 + 1u]; fv.y = pv[c0 + 1u]; }
+                if (c0 + 2u < d) { fk.z = pk[c0 + 2u]; fv.z = pv[c0 + 2u]; }
+                if (c0 + 3u < d) { fk.w = pk[c0 + 3u]; fv.w = pv[c0 + 3u]; }
+            }"""
     src = f"""{PRELUDE}{_CACHE8}
 #define DP {DP}u
 #define C4 {DP // 4}u
-static __device__ __forceinline__ u32 code_of(float x, float s, float inv) {{
-    float q = rintf(x * inv);
-    const float r = fmaf(-q, s, x), r2 = 2.0f * fabsf(r);
-    if (r2 > s || (r2 == s && ((int)q & 1))) q += r < 0.0f ? -1.0f : 1.0f;
-    return (u32)((int)fminf(fmaxf(q, -127.0f), 127.0f) + 128);
+// four codes + 128 in the bytes of a word
+static __device__ __forceinline__ u32 codes_of(float4 f, float s, float inv, float up) {{
+    const float x[4] = {{f.x * up, f.y * up, f.z * up, f.w * up}};
+    float q[4], far = 0.0f;
+    #pragma unroll
+    for (u32 i = 0; i < 4u; ++i) {{
+        const float z = x[i] * inv;                                     // off by 127 * 2^-23 at most
+        q[i] = rintf(z);
+        far = fmaxf(far, fabsf(z - q[i]));
+    }}
+    if (far > 0.49998f) {{                                              // next to a half: the remainder decides
+        #pragma unroll
+        for (u32 i = 0; i < 4u; ++i) {{
+            const float r = fmaf(-q[i], s, x[i]), r2 = 2.0f * fabsf(r);
+            if (r2 > s || (r2 == s && ((int)q[i] & 1))) q[i] += r < 0.0f ? -1.0f : 1.0f;
+        }}
+    }}
+    u32 w = 0u;
+    #pragma unroll
+    for (u32 i = 0; i < 4u; ++i) w |= (u32)(fminf(fmaxf(q[i], -127.0f), 127.0f) + 128.0f) << (8u * i);
+    return w;
 }}
+static __device__ __forceinline__ float most4(float4 f) {{ return fmaxf(fmaxf(fabsf(f.x), fabsf(f.y)), fmaxf(fabsf(f.z), fabsf(f.w))); }}
 static __device__ __forceinline__ bool odd_one(float x) {{ return !(fabsf(x) < __builtin_inff()); }}
-extern "C" __global__ __launch_bounds__(256) void {name}(const float* __restrict__ k, const float* __restrict__ v,
+static __device__ __forceinline__ bool odd4(float4 f) {{ return odd_one(f.x) || odd_one(f.y) || odd_one(f.z) || odd_one(f.w); }}
+extern "C" __global__ __launch_bounds__({NT}) void {name}(const float* __restrict__ k, const float* __restrict__ v,
         const float* __restrict__ lengths, const float* __restrict__ counts,
         unsigned char* __restrict__ kc, unsigned char* __restrict__ vc, float* __restrict__ scales, float* tail_k, float* tail_v,
         u32 T, u32 H, u32 d, u32 NB, u32 kp, u32 vp) {{
-    __shared__ __attribute__((aligned(16))) u32 vt[DP * 16u];       // value codes of the block, [DP][64] bytes
-    __shared__ float sk[4], sv[4];
+    __shared__ u32 vt[DP * 17u];                                        // value codes of the block, rows of 64 bytes, 68 apart
+    __shared__ float sk[{NT // 64}], sv[{NT // 64}];
     __shared__ u32 bad[64];
     const u32 t = threadIdx.x, lane = t & 63u, h = blockIdx.y, b = blockIdx.z;
     u32 len, n;
@@ -299,7 +351,7 @@ extern "C" __global__ __launch_bounds__(256) void {name}(const float* __restrict
     const float* __restrict__ vh = v + (u64)b * T * vp + (u64)h * d;
     for (u32 pass = 0; pass < 2u; ++pass) {{
         const u32 blk = pass ? last : first + blockIdx.x;
-        if (pass && (blockIdx.x != 0u || last == first)) break;            // (uniform over the workgroup)
+        if (pass && (blockIdx.x != 0u || last == first || !(total & 63u))) break;       // (uniform over the workgroup)
         const bool full = blk < last;
         if (!pass && !full && blk != first) break;
         if (blk >= NB) break;
@@ -308,34 +360,21 @@ extern "C" __global__ __launch_bounds__(256) void {name}(const float* __restrict
         const u32 lo = blk == first ? (len & 63u) : 0u, hi = full ? 64u : (total & 63u);       // new rows of this block
         if (t < 64u) bad[t] = 0u;
         __syncthreads();
-        float xk[{IT}][4][4], xv[{IT}][4][4];
+        float4 xk[{IT}], xv[{IT}];
         float mk = 0.0f, mv = 0.0f;
         #pragma unroll
         for (u32 it = 0; it < {IT}u; ++it) {{
-            const u32 item = it * 256u + t, c0 = (item % C4) * 4u, tq = item / C4;
-            #pragma unroll
-            for (u32 i = 0; i < 4u; ++i) {{
-                const u32 row = tq * 4u + i;
-                float4 fk = make_float4(0.f, 0.f, 0.f, 0.f), fv = fk;
-                if (tq < 16u && row < hi) {{
-                    if (row < lo) {{                                           // from the tail (only the block the call starts in)
-                        if (full) {{
-                            fk = *reinterpret_cast<const float4*>(tk + row * DP + c0);
-                            fv = *reinterpret_cast<const float4*>(tv + row * DP + c0);
-                        }}
-                    }} else if (c0 < d) {{
-                        const u64 at = (u64)blk * 64u + row - len;
-                        {{ const float* __restrict__ src = kh + at * kp; {ld} fk = f; }}
-                        {{ const float* __restrict__ src = vh + at * vp; {ld} fv = f; }}
-                    }}
-                    if (odd_one(fk.x) || odd_one(fk.y) || odd_one(fk.z) || odd_one(fk.w) || odd_one(fv.x) || odd_one(fv.y) || odd_one(fv.z) || odd_one(fv.w))
-                        bad[row] = 1u;
-                }}
-                xk[it][i][0] = fk.x; xk[it][i][1] = fk.y; xk[it][i][2] = fk.z; xk[it][i][3] = fk.w;
-                xv[it][i][0] = fv.x; xv[it][i][1] = fv.y; xv[it][i][2] = fv.z; xv[it][i][3] = fv.w;
-                mk = fmaxf(mk, fmaxf(fmaxf(fabsf(fk.x), fabsf(fk.y)), fmaxf(fabsf(fk.z), fabsf(fk.w))));
-                mv = fmaxf(mv, fmaxf(fmaxf(fabsf(fv.x), fabsf(fv.y)), fmaxf(fabsf(fv.z), fabsf(fv.w))));
-            }}
+            const u32 row = (it * {NT}u + t) / C4, c0 = (it * {NT}u + t) % C4 * 4u;
+            // a row of the block: new, or from the tail (only the block the call starts in, and only if it is quantised now)
+            const bool there = row < hi && (row >= lo || full);
+            const u64 at = (u64)blk * 64u + row - len;
+            float4 fk = make_float4(0.f, 0.f, 0.f, 0.f), fv = fk;
+            {load}
+            if (odd4(fk) || odd4(fv)) bad[row] = 1u;
+            xk[it] = fk;
+            xv[it] = fv;
+            mk = fmaxf(mk, most4(fk));
+            mv = fmaxf(mv, most4(fv));
         }}
         mk = wave_max(mk);
         mv = wave_max(mv);
@@ -345,55 +384,42 @@ extern "C" __global__ __launch_bounds__(256) void {name}(const float* __restrict
         if (!full || (blk == first && last == first + 1u)) {{
             #pragma unroll
             for (u32 it = 0; it < {IT}u; ++it) {{
-                const u32 item = it * 256u + t, c0 = (item % C4) * 4u, tq = item / C4;
-                #pragma unroll
-                for (u32 i = 0; i < 4u; ++i) {{
-                    const u32 row = tq * 4u + i;
-                    if (tq < 16u && row >= lo && row < hi) {{
-                        const float z = bad[row] ? __builtin_nanf("") : 0.0f;
-                        float4 fk = make_float4(xk[it][i][0], xk[it][i][1], xk[it][i][2], xk[it][i][3]);
-                        float4 fv = make_float4(xv[it][i][0], xv[it][i][1], xv[it][i][2], xv[it][i][3]);
-                        if (z != z) {{ fk = make_float4(z, z, z, z); fv = fk; }}
-                        *reinterpret_cast<float4*>(tk + row * DP + c0) = fk;
-                        *reinterpret_cast<float4*>(tv + row * DP + c0) = fv;
-                    }}
+                const u32 row = (it * {NT}u + t) / C4, c0 = (it * {NT}u + t) % C4 * 4u;
+                if (row >= lo && row < hi) {{
+                    const float z = __builtin_nanf("");
+                    const bool odd = bad[row] != 0u;
+                    *reinterpret_cast<float4*>(tk + row * DP + c0) = odd ? make_float4(z, z, z, z) : xk[it];
+                    *reinterpret_cast<float4*>(tv + row * DP + c0) = odd ? make_float4(z, z, z, z) : xv[it];
                 }}
             }}
         }}
         if (full) {{
             const bool odd = __any(bad[lane] != 0u);
-            const float ak = fmaxf(fmaxf(sk[0], sk[1]), fmaxf(sk[2], sk[3])) / 127.0f, av = fmaxf(fmaxf(sv[0], sv[1]), fmaxf(sv[2], sv[3])) / 127.0f;
+            float ak = 0.0f, av = 0.0f;
+            #pragma unroll
+            for (u32 i = 0; i < {NT // 64}u; ++i) {{ ak = fmaxf(ak, sk[i]); av = fmaxf(av, sv[i]); }}
+            ak /= 127.0f;
+            av /= 127.0f;
             const u64 at = bh * NB + blk;
-            if (t == 0u) {{
-                scales[2u * at] = odd ? __builtin_nanf("") : ak;
-                scales[2u * at + 1u] = odd ? __builtin_nanf("") : av;
-            }}
+            if (t == 0u) *reinterpret_cast<float2*>(scales + 2u * at) = odd ? make_float2(__builtin_nanf(""), __builtin_nanf("")) : make_float2(ak, av);
             // a scale below 2^-60 has no finite reciprocal or an inexact remainder: both sides times 2^64, exactly
             const float upk = ak < 8.6736174e-19f ? 18446744073709551616.0f : 1.0f, upv = av < 8.6736174e-19f ? 18446744073709551616.0f : 1.0f;
             const float s_k = ak * upk, s_v = av * upv, ik = ak > 0.0f ? 1.0f / s_k : 0.0f, iv = av > 0.0f ? 1.0f / s_v : 0.0f;
             unsigned char* __restrict__ kb = kc + at * (64u * DP);
+            unsigned char* vt8 = reinterpret_cast<unsigned char*>(vt);
             #pragma unroll
             for (u32 it = 0; it < {IT}u; ++it) {{
-                const u32 item = it * 256u + t, c0 = (item % C4) * 4u, tq = item / C4;
-                if (tq < 16u) {{
-                    u32 cv[4] = {{0u, 0u, 0u, 0u}};
+                const u32 row = (it * {NT}u + t) / C4, c0 = (it * {NT}u + t) % C4 * 4u;
+                if (row < 64u) {{
+                    *reinterpret_cast<u32*>(kb + row * DP + c0) = codes_of(xk[it], s_k, ik, upk);
+                    const u32 cv = codes_of(xv[it], s_v, iv, upv);
                     #pragma unroll
-                    for (u32 i = 0; i < 4u; ++i) {{
-                        u32 ck = 0u;
-                        #pragma unroll
-                        for (u32 c = 0; c < 4u; ++c) {{
-                            ck |= ((ak > 0.0f && !odd) ? code_of(xk[it][i][c] * upk, s_k, ik) : 128u) << (8u * c);
-                            cv[c] |= ((av > 0.0f && !odd) ? code_of(xv[it][i][c] * upv, s_v, iv) : 128u) << (8u * i);
-                        }}
-                        *reinterpret_cast<u32*>(kb + (tq * 4u + i) * DP + c0) = ck;
-                    }}
-                    #pragma unroll
-                    for (u32 c = 0; c < 4u; ++c) vt[(c0 + c) * 16u + tq] = cv[c];
+                    for (u32 c = 0; c < 4u; ++c) vt8[(c0 + c) * 68u + row] = (unsigned char)(cv >> (8u * c));
                 }}
             }}
             __syncthreads();
-            uint4* __restrict__ vb = reinterpret_cast<uint4*>(vc + at * (64u * DP));
-            for (u32 i = t; i < DP * 4u; i += 256u) vb[i] = reinterpret_cast<const uint4*>(vt)[i];
+            u32* __restrict__ vb = reinterpret_cast<u32*>(vc + at * (64u * DP));
+            for (u32 i = t; i < DP * 16u; i += {NT}u) vb[i] = vt[(i >> 4) * 17u + (i & 15u)];
         }}
         __syncthreads();
     }}
@@ -430,17 +456,32 @@ extern "C" __global__ __launch_bounds__(256) void {name}(const unsigned char* __
     __syncthreads();
     const float* __restrict__ tk = tail_k + (((u64)(blk & 1u) * heads + bh) * 64u) * DP;
     const float* __restrict__ tv = tail_v + (((u64)(blk & 1u) * heads + bh) * 64u) * DP;
-    for (u32 i = t; i < 64u * d; i += 256u) {{
-        const u32 row = i / d, c = i % d, p = blk * 64u + row;
-        if (p >= N) break;
-        float x = 0.0f, y = 0.0f;
+    const u64 C = (u64)H * d;
+    // four columns a thread (as many of them as there are)
+    for (u32 i = t; i < 64u * {DP // 4}u; i += 256u) {{
+        const u32 row = i / {DP // 4}u, c = i % {DP // 4}u * 4u, p = blk * 64u + row;
+        if (p >= N || c >= d) continue;
+        float4 x = make_float4(0.f, 0.f, 0.f, 0.f), z = x;
         if (blk < last) {{
-            x = (float)((int)kb[row * DP + c] - 128) * s_k;
-            y = (float)((int)reinterpret_cast<const unsigned char*>(vt)[c * 68u + row] - 128) * s_v;
-        }} else if (p < total) {{ x = tk[row * DP + c]; y = tv[row * DP + c]; }}
-        const u64 o = ((u64)b * N + p) * ((u64)H * d) + (u64)h * d + c;
-        ko[o] = x;
-        vo[o] = y;
+            const u32 w = *reinterpret_cast<const u32*>(kb + row * DP + c);
+            const unsigned char* vt8 = reinterpret_cast<const unsigned char*>(vt) + c * 68u + row;
+            x = make_float4((float)((int)(w & 255u) - 128) * s_k, (float)((int)((w >> 8) & 255u) - 128) * s_k,
+                            (float)((int)((w >> 16) & 255u) - 128) * s_k, (float)((int)(w >> 24) - 128) * s_k);
+            z = make_float4((float)((int)vt8[0] - 128) * s_v, (float)((int)vt8[68] - 128) * s_v, (float)((int)vt8[136] - 128) * s_v, (float)((int)vt8[204] - 128) * s_v);
+        }} else if (p < total) {{
+            x = *reinterpret_cast<const float4*>(tk + row * DP + c);
+            z = *reinterpret_cast<const float4*>(tv + row * DP + c);
+        }}
+        const u64 o = ((u64)b * N + p) * C + (u64)h * d + c;
+        if ((d & 3u) == 0u) {{                                              // (fresh results are aligned)
+            *reinterpret_cast<float4*>(ko + o) = x;
+            *reinterpret_cast<float4*>(vo + o) = z;
+        }} else {{
+            ko[o] = x.x; vo[o] = z.x;
+            if (c + 1u < d) {{ ko[o + 1u] = x.y; vo[o + 1u] = z.y; }}
+            if (c + 2u < d) {{ ko[o + 2u] = x.z; vo[o + 2u] = z.z; }}
+            if (c + 3u < d) {{ ko[o + 3u] = x.w; vo[o + 3u] = z.w; }}
+        }}
     }}
 }}
 """
@@ -448,7 +489,7 @@ extern "C" __global__ __launch_bounds__(256) void {name}(const unsigned char* __
 
 
 @cache
-def cache8_attend_kernel(DP: int) -> tuple[str, str, str]:
+def cache8_attend_kernel(DP: int, NQ: int = 1, W: int = 4, stream: bool = False) -> tuple[str, str, str]:
     """Attention of T new positions per sequence over the 8-bit cache of one layer, after their keys and values were written:
     y = softmax(q K^T * scale) V per query head, query t of sequence b at position lengths[b] + t seeing the positions up to its
     own; `group` query heads share a key head.  q and y are (B, T, H * group * d).  A row beyond counts[b] gives zeros.
@@ -456,27 +497,41 @@ def cache8_attend_kernel(DP: int) -> tuple[str, str, str]:
     The codes are whole numbers of at most 127 and therefore exact in 16-bit floats, so the matrix units do the work:
     a query row is scaled by a power of two to at most 2^15 and cut into two 16-bit floats, q' = q1 + q2 (22 bits and more of
     it), and S^T = K (q1 + q2)^T has fp32 accuracy from two v_mfma_f32_16x16x32_f16 per 32 columns.  The probabilities go the
-    same way: p' = 2^15 exp(s - m) = p1 + p2, the factor cancels in p' V / sum p'.  The scales enter in 32 bits, the keys'
-    with the scores, the values' as a block's product joins the running sum.
+    same way: p' = 2^15 exp(s - m) = p1 + p2 (p1 rounded to nearest, the rest, of either sign, cut off after 11 bits: 2^-22 of p'),
+    and the factor cancels in p' V / sum p'.  The scales enter in 32 bits, the keys' with the scores, the values' as a block's
+    product joins the running sum.
 
-    A wavefront takes one block of 64 tokens at a time, with (m, l, O) of its own per query.  Its lane r + 16 g (r, g < 16, 4) holds
-    query r and, of every product S^T, four tokens; the rows of K are fed in the order that makes those of the four tiles the
-    sixteen neighbours 16 g ..: then P is already the B operand of O^T += V^T P^T, and its A operand, sixteen value codes
-    of one column, is one 16-byte load from the transposed block.  Nothing passes through LDS.  Bytes become 16-bit floats in one
-    operation each: v_perm puts byte c under the exponent of 1024, giving 1024 + c, and a packed addition takes 1152 away.
+    A wavefront takes one block of 64 tokens at a time, for NQ tiles of 16 query rows, with (m, l, O) of its own.  Its lane
+    r + 16 g (r < 16, g < 4) holds query r of each tile and, of every product S^T, four tokens; the rows of K are fed in the order
+    that makes those of the four token tiles the sixteen neighbours 16 g ..: then P is already the B operand of O^T += V^T P^T,
+    and its A operand, sixteen value codes of one column, is one 16-byte load from the transposed block.  Nothing passes through
+    LDS.  Bytes become 16-bit floats in one operation each: v_perm puts byte c under the exponent of 1024, giving 1024 + c, and
+    a packed addition takes 1152 away.  The keys of the next block are loaded when those of this one have been used, while its
+    softmax runs, and its values likewise during the next scores.  stream: loads that leave no trace in the caches, for codes that
+    are read once and would only displace others.
 
     The tail, fp32, is shared out 16 tokens to a wavefront and goes through v_mfma_f32_16x16x4_f32.
 
-    A workgroup of four wavefronts per (16 query rows of one key head, split of the blocks); the four are joined through LDS in
+    A workgroup of W wavefronts per (NQ tiles of one key head, split of the blocks); they are joined through LDS in
     wavefront order.  With one split y is written; else O, m and l go to `part` and cache8_join_kernel adds the splits up
-    in their order.  Bound by memory while few query rows share a key head: 2 bytes per token and column."""
+    in their order.  Bound by memory while few query rows share a key head: 2 bytes per token and column.  With many, by
+    the vector units: about 2 operations per score and code against a matrix instruction's 1/16."""
     ND, NK, Q4 = DP // 16, DP // 32, DP // 4             # column tiles of V^T, k steps of a score, columns a lane feeds
-    name = f"cache8_attend_d{DP}"
+    name = f"cache8_attend_d{DP}" + (f"_q{NQ}" if NQ > 1 else "") + (f"_w{W}" if W != 4 else "") + ("_nt" if stream else "")
+    fetch = "__builtin_nontemporal_load({})" if stream else "*{}"
+    fetch2, fetch4 = (fetch.format(f"reinterpret_cast<const u{n}*>({at})") for n, at in ((2, "p + 4u * u * DP + 8u * i"), (4, "p + dt * 1024u")))
     kw = Q4 // 8                                          # 8-byte words of a key row per lane
+    # "256, 2" holds the kernel to 256 registers, with which the matrix instructions write ordinary ones; wider heads need more
+    bounds = "256, 2" if W == 4 and DP * NQ <= 128 else f"{64 * W}"
     src = f"""{PRELUDE}{_CACHE8}
 #define DP {DP}u
 #define ND {ND}u
 #define NK {NK}u
+#define NQ {NQ}u
+#define W {W}u
+typedef u32 u2 __attribute__((ext_vector_type(2)));
+typedef u32 u4 __attribute__((ext_vector_type(4)));
+typedef float f2 __attribute__((ext_vector_type(2)));
 typedef float f4 __attribute__((ext_vector_type(4)));
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
@@ -496,196 +551,261 @@ static __device__ __forceinline__ h8 widen(u32 lo, u32 hi) {{
     for (int i = 0; i < 4; ++i) r.p[i] += off;
     return r.v;
 }}
-extern "C" __global__ __launch_bounds__(256) void {name}(const float* __restrict__ q, const unsigned char* __restrict__ kc,
+// two numbers as the sum of two pairs of 16-bit floats; minus is -1 where the compiler does not see it: the subtraction
+// then takes the 16-bit float as it is, in one mixed multiply-add
+static __device__ __forceinline__ void halves(float a, float b, float minus, h2& hi, u32& lo) {{
+    const f2 x = {{a, b}};
+    hi = __builtin_convertvector(x, h2);
+    lo = __builtin_bit_cast(u32, __builtin_amdgcn_cvt_pkrtz(fmaf((float)hi.x, minus, a), fmaf((float)hi.y, minus, b)));
+}}
+// the largest of the four lanes r, r + 16, r + 32, r + 48: the swaps leave one half of a pair in each operand
+static __device__ __forceinline__ float four_max(float x) {{
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}}
+struct Inside {{ static constexpr bool edge = false; }};
+struct Edge {{ static constexpr bool edge = true; }};
+extern "C" __global__ __launch_bounds__({bounds}) void {name}(const float* __restrict__ q, const unsigned char* __restrict__ kc,
         const unsigned char* __restrict__ vc, const float* __restrict__ scales, const float* __restrict__ tail_k, const float* __restrict__ tail_v,
         const float* __restrict__ lengths, const float* __restrict__ counts, float* __restrict__ y, float* __restrict__ part,
         u32 B, u32 T, u32 H, u32 group, u32 d, u32 NB, u32 tiles, u32 splits, float scale) {{
-    __shared__ float so[4][16][DP + 4u];
-    __shared__ float sm[4][16], sl[4][16];
-    const u32 t = threadIdx.x, w = t >> 6, lane = t & 63u, r = lane & 15u, g = lane >> 4;
-    const u32 split = blockIdx.x % splits, tile = (blockIdx.x / splits) % tiles;
-    const u32 bh = blockIdx.x / splits / tiles, b = bh / H, h = bh % H;
+    __shared__ float so[W][16][DP + 4u];
+    __shared__ float sm[W][16], sl[W][16];
+    const u32 t = threadIdx.x, w = __builtin_amdgcn_readfirstlane(t >> 6), lane = t & 63u, r = lane & 15u, g = lane >> 4;
+    // workgroups go round the eight dies: all of a key head's on one, whose L2 then holds its codes once
+    const u32 per = tiles * splits, spread = (B * H) % 8u == 0u ? 8u : 1u, at0 = blockIdx.x / spread;
+    const u32 bh = (at0 / per) * spread + blockIdx.x % spread, b = bh / H, h = bh % H;
+    const u32 split = at0 % splits, tile = (at0 / splits) % tiles;
     u32 len, n;
     cache8_extent(lengths, counts, b, T, NB * 64u, len, n);
     const u32 rows = T * group, last = (len + n) >> 6;                       // blocks below `last` are codes
-    const u32 row = tile * 16u + r, tq = row / group;
-    const bool live = row < rows && tq < n;
-    const u32 see = live ? len + tq + 1u : 0u;                                 // positions this lane's query sees
-    const u32 tile_last = min(min(tile * 16u + 15u, rows - 1u) / group, n ? n - 1u : 0u);
-    const u32 most = (n && tile * 16u / group < n) ? len + tile_last + 1u : 0u;               // ... and the last query of the tile
-    const u32 least = min(tile * 16u + 15u, rows - 1u) / group < n ? len + tile * 16u / group + 1u : 0u;   // ... and the first (a padded row: none)
+    const u32 row0 = tile * (16u * NQ), row1 = min(row0 + 16u * NQ, rows) - 1u, t0 = row0 / group, t1 = row1 / group;
+    const u32 most = t0 < n ? len + min(t1, n - 1u) + 1u : 0u;                   // positions that the last query of the tiles sees
+    const u32 least = t1 < n ? len + t0 + 1u : 0u;                              // ... and the first (a padded row: none)
     const u64 C = (u64)H * group * d;
-    const float* __restrict__ qrow = q + ((u64)b * T + tq) * C + (u64)(h * group + row % group) * d;
-    // this lane's quarter of its query row, as two 16-bit floats an element
-    H8 q1[NK], q2[NK];
-    float back;
-    {{
+    const float l2 = fabsf(scale) * 1.44269504088896340736f;
+    float minus = -1.0f;
+    asm volatile("" : "+v"(minus));
+    // this lane's quarter of its query rows, as two 16-bit floats an element; the sign of the scale goes with them
+    H8 q1[NQ][NK], q2[NQ][NK];
+    float back[NQ];
+    u32 see[NQ];                                                              // positions this lane's queries see
+    const float* qrow[NQ];
+    #pragma unroll
+    for (u32 a = 0; a < NQ; ++a) {{
+        const u32 row = row0 + 16u * a + r, tq = row / group;
+        const bool live = row < rows && tq < n;
+        see[a] = live ? len + tq + 1u : 0u;
+        qrow[a] = q + ((u64)b * T + (live ? tq : 0u)) * C + (u64)(h * group + row % group) * d;
         float f[{Q4}], mx = 0.0f;
         #pragma unroll
         for (u32 i = 0; i < {Q4}u; ++i) {{
             const u32 c = g * {Q4}u + i;
-            f[i] = (live && c < d) ? qrow[c] : 0.0f;
+            f[i] = (live && c < d) ? qrow[a][c] : 0.0f;
             mx = fmaxf(mx, fabsf(f[i]));
         }}
-        mx = fmaxf(mx, __shfl_xor(mx, 16, WAVE));
-        mx = fmaxf(mx, __shfl_xor(mx, 32, WAVE));
+        mx = four_max(mx);
         const int e = max((int)((__float_as_uint(mx) >> 23) & 255u), 27) - 127;      // 2^e <= mx < 2^(e + 1)
-        const float up = __uint_as_float((u32)(14 - e + 127) << 23);
-        back = __uint_as_float((u32)(e - 14 + 127) << 23) * (scale * 1.44269504088896340736f);
+        const float up = copysignf(__uint_as_float((u32)(14 - e + 127) << 23), scale);
+        back[a] = __uint_as_float((u32)(e - 14 + 127) << 23) * l2;
         #pragma unroll
-        for (u32 i = 0; i < {Q4}u; ++i) {{
-            const float z = f[i] * up;
-            q1[i >> 3].e[i & 7u] = (_Float16)z;
-            q2[i >> 3].e[i & 7u] = (_Float16)(z - (float)q1[i >> 3].e[i & 7u]);
-        }}
+        for (u32 i = 0; i < {Q4 // 2}u; ++i) halves(f[2u * i] * up, f[2u * i + 1u] * up, minus, q1[a][i >> 2].p[i & 3u], q2[a][i >> 2].w[i & 3u]);
     }}
-    f4 o[ND];
+    f4 o[NQ][ND];
+    float m[NQ], l[NQ];
     #pragma unroll
-    for (u32 dt = 0; dt < ND; ++dt) o[dt] = (f4){{0.f, 0.f, 0.f, 0.f}};
-    float m = NINF, l = 0.0f;
-    const u32 nb = min(last, (most + 63u) >> 6);                                    // blocks of codes that the tile sees
-    const u32 j0 = (u32)((u64)nb * split / splits), j1 = (u32)((u64)nb * (split + 1u) / splits);
+    for (u32 a = 0; a < NQ; ++a) {{
+        m[a] = NINF; l[a] = 0.0f;
+        #pragma unroll
+        for (u32 dt = 0; dt < ND; ++dt) o[a][dt] = (f4){{0.f, 0.f, 0.f, 0.f}};
+    }}
+    const u32 nb = min(last, (most + 63u) >> 6);                                    // blocks of codes that the tiles see
+    const u32 j0 = (u32)((u64)nb * split / splits) + w, j1 = (u32)((u64)nb * (split + 1u) / splits);
     const u64 base = ((u64)bh * NB) * (64u * DP);
-    const u32 k_at = (16u * (r >> 2) + (r & 3u)) * DP + g * {Q4}u;              // + 4 u DP for tile u
-    const u32 v_at = r * 64u + g * 16u;                                         // + dt 16 * 64
-    for (u32 j = j0 + w; j < j1; j += 4u) {{
-        const unsigned char* __restrict__ kb = kc + base + (u64)j * (64u * DP) + k_at;
-        const unsigned char* __restrict__ vb = vc + base + (u64)j * (64u * DP) + v_at;
-        uint2 kr[4][{kw}];
-        uint4 vr[ND];
+    const unsigned char* __restrict__ kh = kc + base + (16u * (r >> 2) + (r & 3u)) * DP + g * {Q4}u;     // + 4 u DP for token tile u
+    const unsigned char* __restrict__ vh = vc + base + r * 64u + g * 16u;                              // + 1024 dt for column tile dt
+    const float2* __restrict__ sh = reinterpret_cast<const float2*>(scales) + (u64)bh * NB;
+    u2 kr[4][{kw}];
+    u4 vr[ND];
+    float2 sc;
+    auto load_k = [&](u32 j) {{
+        const unsigned char* __restrict__ p = kh + (u64)j * (64u * DP);
         #pragma unroll
         for (u32 u = 0; u < 4u; ++u)
             #pragma unroll
-            for (u32 i = 0; i < {kw}u; ++i) kr[u][i] = *reinterpret_cast<const uint2*>(kb + 4u * u * DP + 8u * i);
+            for (u32 i = 0; i < {kw}u; ++i) kr[u][i] = {fetch2};
+    }};
+    auto load_v = [&](u32 j) {{
+        const unsigned char* __restrict__ p = vh + (u64)j * (64u * DP);
         #pragma unroll
-        for (u32 dt = 0; dt < ND; ++dt) vr[dt] = *reinterpret_cast<const uint4*>(vb + dt * 1024u);
-        const float2 sc = *reinterpret_cast<const float2*>(scales + 2u * ((u64)bh * NB + j));
-        float s[16];
-        const float f = back * sc.x;
+        for (u32 dt = 0; dt < ND; ++dt) vr[dt] = {fetch4};
+    }};
+    if (j0 < j1) {{ load_k(j0); sc = sh[j0]; load_v(j0); }}
+    auto block = [&](u32 j, auto kind) {{
+        constexpr bool edge = decltype(kind)::edge;                                 // some query does not see all of the block
+        const u32 jn = j + W < j1 ? j + W : j;                                     // (the last one is loaded again)
+        f4 s[NQ][4];
         #pragma unroll
         for (u32 u = 0; u < 4u; ++u) {{
-            f4 acc = (f4){{0.f, 0.f, 0.f, 0.f}};
+            #pragma unroll
+            for (u32 a = 0; a < NQ; ++a) s[a][u] = (f4){{0.f, 0.f, 0.f, 0.f}};
             #pragma unroll
             for (u32 i = 0; i < NK; ++i) {{
-                const h8 a = widen(kr[u][i].x, kr[u][i].y);
-                acc = MFMA16(a, q2[i].v, acc);
-                acc = MFMA16(a, q1[i].v, acc);
+                const h8 k8 = widen(kr[u][i].x, kr[u][i].y);
+                #pragma unroll
+                for (u32 a = 0; a < NQ; ++a) {{
+                    s[a][u] = MFMA16(k8, q2[a][i].v, s[a][u]);
+                    s[a][u] = MFMA16(k8, q1[a][i].v, s[a][u]);
+                }}
             }}
-            #pragma unroll
-            for (u32 i = 0; i < 4u; ++i) s[4u * u + i] = acc[i] * f;
         }}
-        if (j * 64u + 64u > least) {{                                               // some query of the tile does not see all of the block
-            #pragma unroll
-            for (u32 i = 0; i < 16u; ++i) if (j * 64u + 16u * g + i >= see) s[i] = NINF;
-        }}
-        float mx = s[0];
+        const float2 now = sc;
+        load_k(jn);
+        sc = sh[jn];
+        const u32 at = j * 64u + 16u * g;
+        const float vs = now.y == now.y ? now.y : 0.0f;                            // (a NaN scale makes the scores NaN as well)
+        H8 p1[NQ][2], p2[NQ][2];
         #pragma unroll
-        for (u32 i = 1; i < 16u; ++i) mx = fmaxf(mx, s[i]);
-        mx = fmaxf(mx, __shfl_xor(mx, 16, WAVE));
-        mx = fmaxf(mx, __shfl_xor(mx, 32, WAVE));
-        const float mn = fmaxf(m, mx), mu = mn == NINF ? 0.0f : mn, alpha = __builtin_amdgcn_exp2f(m - mu);
-        m = mn;
-        float sum = 0.0f;
-        H8 p1[2], p2[2];
-        #pragma unroll
-        for (u32 i = 0; i < 16u; ++i) {{
-            const float p = __builtin_amdgcn_exp2f(s[i] - mu + 15.0f);
-            sum += p;
-            p1[i >> 3].e[i & 7u] = (_Float16)p;
-            p2[i >> 3].e[i & 7u] = (_Float16)(p - (float)p1[i >> 3].e[i & 7u]);
+        for (u32 a = 0; a < NQ; ++a) {{
+            if constexpr (edge) {{
+                #pragma unroll
+                for (u32 i = 0; i < 16u; ++i) if (at + i >= see[a]) s[a][i >> 2][i & 3u] = NEG_FLT_MAX;
+            }}
+            float mx = s[a][0][0];
+            #pragma unroll
+            for (u32 i = 1; i < 16u; ++i) mx = fmaxf(mx, s[a][i >> 2][i & 3u]);
+            mx = four_max(mx);
+            const float f = back[a] * now.x;                                        // not negative: the maximum stays one
+            const float mn = fmaxf(m[a], mx * f), mu = mn == NINF ? 0.0f : mn;
+            if (__any(mn != m[a])) {{                                               // (a maximum that stays is the rule after the first blocks)
+                const float alpha = __builtin_amdgcn_exp2f(m[a] - mu);
+                m[a] = mn;
+                l[a] *= alpha;
+                #pragma unroll
+                for (u32 dt = 0; dt < ND; ++dt) o[a][dt] *= alpha;
+            }}
+            float sum = 0.0f;
+            #pragma unroll
+            for (u32 i = 0; i < 16u; i += 2u) {{
+                float p = __builtin_amdgcn_exp2f(fmaf(s[a][i >> 2][i & 3u], f, 15.0f - mu));
+                float z = __builtin_amdgcn_exp2f(fmaf(s[a][i >> 2][(i & 3u) + 1u], f, 15.0f - mu));
+                if constexpr (edge) {{ p = at + i < see[a] ? p : 0.0f; z = at + i + 1u < see[a] ? z : 0.0f; }}
+                sum += p + z;
+                halves(p, z, minus, p1[a][i >> 3].p[(i & 7u) >> 1], p2[a][i >> 3].w[(i & 7u) >> 1]);
+            }}
+            l[a] += sum;
         }}
-        l = l * alpha + sum;
-        const float vs = sc.y == sc.y ? sc.y : 0.0f;                               // (a NaN scale has made the scores NaN already)
         #pragma unroll
         for (u32 dt = 0; dt < ND; ++dt) {{
-            f4 acc = (f4){{0.f, 0.f, 0.f, 0.f}};
-            const h8 a0 = widen(vr[dt].x, vr[dt].y), a1 = widen(vr[dt].z, vr[dt].w);
-            acc = MFMA16(a0, p2[0].v, acc);
-            acc = MFMA16(a1, p2[1].v, acc);
-            acc = MFMA16(a0, p1[0].v, acc);
-            acc = MFMA16(a1, p1[1].v, acc);
+            const h8 v0 = widen(vr[dt].x, vr[dt].y), v1 = widen(vr[dt].z, vr[dt].w);
             #pragma unroll
-            for (u32 i = 0; i < 4u; ++i) o[dt][i] = o[dt][i] * alpha + vs * acc[i];
+            for (u32 a = 0; a < NQ; ++a) {{
+                f4 acc = (f4){{0.f, 0.f, 0.f, 0.f}};
+                acc = MFMA16(v0, p2[a][0].v, acc);
+                acc = MFMA16(v1, p2[a][1].v, acc);
+                acc = MFMA16(v0, p1[a][0].v, acc);
+                acc = MFMA16(v1, p1[a][1].v, acc);
+                #pragma unroll
+                for (u32 i = 0; i < 4u; ++i) o[a][dt][i] = fmaf(vs, acc[i], o[a][dt][i]);
+            }}
         }}
-    }}
-    if (split == splits - 1u && most > last * 64u + 16u * w) {{                     // sixteen tokens of the tail
+        load_v(jn);
+    }};
+    u32 j = j0;
+    for (; j < j1 && j * 64u + 64u <= least; j += W) block(j, Inside());
+    for (; j < j1; j += W) block(j, Edge());
+    const u32 tt = W - 1u - w;                                                      // sixteen tokens of the tail: the wavefronts with the fewest blocks
+    if (split == splits - 1u && tt < 4u && most > last * 64u + 16u * tt) {{
         const u64 heads = (u64)B * H;
-        const float* __restrict__ tk = tail_k + (((u64)(last & 1u) * heads + bh) * 64u + 16u * w) * DP;
-        const float* __restrict__ tv = tail_v + (((u64)(last & 1u) * heads + bh) * 64u + 16u * w) * DP;
-        f4 acc = (f4){{0.f, 0.f, 0.f, 0.f}};
+        const float* __restrict__ tk = tail_k + (((u64)(last & 1u) * heads + bh) * 64u + 16u * tt) * DP;
+        const float* __restrict__ tv = tail_v + (((u64)(last & 1u) * heads + bh) * 64u + 16u * tt) * DP;
+        const u32 p0 = last * 64u + 16u * tt + 4u * g;                              // this lane's four tokens
+        float kt[{Q4}], vt[ND][4];                                                  // (both on their way before the first is used)
         #pragma unroll
-        for (u32 i = 0; i < {Q4}u; ++i) {{
-            const u32 c = g * {Q4}u + i;
-            acc = MFMA32(tk[r * DP + c], (live && c < d) ? qrow[c] : 0.0f, acc);
-        }}
-        const u32 p0 = last * 64u + 16u * w + 4u * g;                               // this lane's four tokens
-        float mx = NINF;
+        for (u32 i = 0; i < {Q4}u; ++i) kt[i] = tk[r * DP + g * {Q4}u + i];
         #pragma unroll
-        for (u32 i = 0; i < 4u; ++i) {{
-            acc[i] = p0 + i < see ? acc[i] * (scale * 1.44269504088896340736f) : NINF;
-            mx = fmaxf(mx, acc[i]);
-        }}
-        mx = fmaxf(mx, __shfl_xor(mx, 16, WAVE));
-        mx = fmaxf(mx, __shfl_xor(mx, 32, WAVE));
-        const float mn = fmaxf(m, mx), mu = mn == NINF ? 0.0f : mn, alpha = __builtin_amdgcn_exp2f(m - mu);
-        m = mn;
-        float sum = 0.0f;
-        #pragma unroll
-        for (u32 i = 0; i < 4u; ++i) {{ acc[i] = __builtin_amdgcn_exp2f(acc[i] - mu + 15.0f); sum += acc[i]; }}
-        l = l * alpha + sum;
-        #pragma unroll
-        for (u32 dt = 0; dt < ND; ++dt) {{
+        for (u32 dt = 0; dt < ND; ++dt)
             #pragma unroll
-            for (u32 i = 0; i < 4u; ++i) o[dt][i] *= alpha;
+            for (u32 i = 0; i < 4u; ++i) vt[dt][i] = tv[(4u * g + i) * DP + dt * 16u + r];
+        #pragma unroll
+        for (u32 a = 0; a < NQ; ++a) {{
+            f4 acc = (f4){{0.f, 0.f, 0.f, 0.f}};
+            #pragma unroll
+            for (u32 i = 0; i < {Q4}u; ++i) {{
+                const u32 c = g * {Q4}u + i;
+                acc = MFMA32(kt[i], (see[a] && c < d) ? qrow[a][c] : 0.0f, acc);
+            }}
+            float mx = NINF;
             #pragma unroll
             for (u32 i = 0; i < 4u; ++i) {{
-                const float x = tv[(4u * g + i) * DP + dt * 16u + r];
-                o[dt] = MFMA32((p0 + i < most && x == x) ? x : 0.0f, acc[i], o[dt]);      // (a NaN row has made the scores NaN already)
+                acc[i] = p0 + i < see[a] ? acc[i] * (scale * 1.44269504088896340736f) : NINF;
+                mx = fmaxf(mx, acc[i]);
+            }}
+            mx = four_max(mx);
+            const float mn = fmaxf(m[a], mx), mu = mn == NINF ? 0.0f : mn, alpha = __builtin_amdgcn_exp2f(m[a] - mu);
+            m[a] = mn;
+            float sum = 0.0f;
+            #pragma unroll
+            for (u32 i = 0; i < 4u; ++i) {{ acc[i] = __builtin_amdgcn_exp2f(acc[i] - mu + 15.0f); sum += acc[i]; }}
+            l[a] = l[a] * alpha + sum;
+            #pragma unroll
+            for (u32 dt = 0; dt < ND; ++dt) {{
+                #pragma unroll
+                for (u32 i = 0; i < 4u; ++i) o[a][dt][i] *= alpha;
+                #pragma unroll
+                for (u32 i = 0; i < 4u; ++i) {{
+                    const float x = vt[dt][i];
+                    o[a][dt] = MFMA32((p0 + i < most && x == x) ? x : 0.0f, acc[i], o[a][dt]);  // (a NaN row makes the scores NaN as well)
+                }}
             }}
         }}
     }}
-    l += __shfl_xor(l, 16, WAVE);
-    l += __shfl_xor(l, 32, WAVE);
-    if (g == 0u) {{ sm[w][r] = m; sl[w][r] = l; }}
     #pragma unroll
-    for (u32 dt = 0; dt < ND; ++dt) *reinterpret_cast<f4*>(&so[w][r][dt * 16u + 4u * g]) = o[dt];
-    __syncthreads();
-    // sixteen threads a row: the four wavefronts' parts, in their order
-    const u32 jr = t >> 4, jc = t & 15u, jrow = tile * 16u + jr;
-    if (jrow >= rows) return;
-    float M = NINF, L = 0.0f, fac[4];
-    #pragma unroll
-    for (u32 i = 0; i < 4u; ++i) M = fmaxf(M, sm[i][jr]);
-    #pragma unroll
-    for (u32 i = 0; i < 4u; ++i) {{ fac[i] = sm[i][jr] == NINF ? 0.0f : __builtin_amdgcn_exp2f(sm[i][jr] - M); L += fac[i] * sl[i][jr]; }}
-    if (splits == 1u) {{
-        float* __restrict__ yr = y + ((u64)b * T + jrow / group) * C + (u64)(h * group + jrow % group) * d;
-        for (u32 c = jc; c < d; c += 16u) {{
-            float a = 0.0f;
+    for (u32 a = 0; a < NQ; ++a) {{
+        l[a] += __shfl_xor(l[a], 16, WAVE);
+        l[a] += __shfl_xor(l[a], 32, WAVE);
+        if (a) __syncthreads();                                                     // (the tile before has been read)
+        if (g == 0u) {{ sm[w][r] = m[a]; sl[w][r] = l[a]; }}
+        #pragma unroll
+        for (u32 dt = 0; dt < ND; ++dt) *reinterpret_cast<f4*>(&so[w][r][dt * 16u + 4u * g]) = o[a][dt];
+        __syncthreads();
+        // 4 W threads a row: the wavefronts' parts, in their order
+        const u32 jr = t / (4u * W), jc = t % (4u * W), jrow = row0 + 16u * a + jr;
+        if (jrow < rows) {{
+            float M = NINF, L = 0.0f, fac[W];
             #pragma unroll
-            for (u32 i = 0; i < 4u; ++i) a += fac[i] * so[i][jr][c];
-            yr[c] = L == 0.0f ? 0.0f : a / L;
-        }}
-    }} else {{
-        float* __restrict__ pr = part + (((u64)bh * rows + jrow) * splits + split) * (DP + 2u);
-        for (u32 c = jc; c < d; c += 16u) {{
-            float a = 0.0f;
+            for (u32 i = 0; i < W; ++i) M = fmaxf(M, sm[i][jr]);
             #pragma unroll
-            for (u32 i = 0; i < 4u; ++i) a += fac[i] * so[i][jr][c];
-            pr[c] = a;
+            for (u32 i = 0; i < W; ++i) {{ fac[i] = sm[i][jr] == NINF ? 0.0f : __builtin_amdgcn_exp2f(sm[i][jr] - M); L += fac[i] * sl[i][jr]; }}
+            float* __restrict__ yr = splits == 1u ? y + ((u64)b * T + jrow / group) * C + (u64)(h * group + jrow % group) * d
+                                                  : part + (((u64)bh * rows + jrow) * splits + split) * (DP + 2u);
+            const float inv = splits > 1u ? 1.0f : L == 0.0f ? 0.0f : 1.0f / L;
+            for (u32 c = jc; c < d; c += 4u * W) {{
+                float x = 0.0f;
+                #pragma unroll
+                for (u32 i = 0; i < W; ++i) x += fac[i] * so[i][jr][c];
+                yr[c] = x * inv;
+            }}
+            if (splits > 1u && jc == 0u) {{ yr[DP] = M; yr[DP + 1u] = L; }}
         }}
-        if (jc == 0u) {{ pr[DP] = M; pr[DP + 1u] = L; }}
     }}
 }}
 """
     return src, name, _fmt("P" * 10, "I" * 8, "f")
 
 
+CACHE8_MAX_SPLITS = 64      # what one wavefront joins: a lane per split
+
+
 @cache
 def cache8_join_kernel(DP: int) -> tuple[str, str, str]:
-    """Adds up what cache8_attend_kernel left per split: O = sum exp(m_s - M) O_s over sum exp(m_s - M) l_s, in the order of the
-    splits.  One wavefront per query row of a key head."""
+    """Adds up what cache8_attend_kernel left per split: O = sum exp(m_s - M) O_s over sum exp(m_s - M) l_s.  One wavefront per query
+    row of a key head: lane s takes m and l of split s (at most 64), the factors go round, and the columns are added in the order of
+    the splits with eight loads in flight.  Bound by latency: two dependent reads."""
     name = f"cache8_join_d{DP}"
+    N = (DP + 63) // 64
     src = f"""{PRELUDE}
 #define DP {DP}u
 #define NINF (-__builtin_inff())
@@ -695,21 +815,21 @@ extern "C" __global__ __launch_bounds__(256) void {name}(const float* __restrict
     if (item >= items) return;
     const u32 rows = T * group, bh = item / rows, row = item % rows, b = bh / H, h = bh % H;
     const float* __restrict__ pr = part + (u64)item * splits * (DP + 2u);
-    float M = NINF, L = 0.0f;
-    for (u32 s = 0; s < splits; ++s) M = fmaxf(M, pr[s * (DP + 2u) + DP]);
-    float acc[{(DP + 63) // 64}];
+    const float2 ml = lane < splits ? *reinterpret_cast<const float2*>(pr + lane * (DP + 2u) + DP) : make_float2(NINF, 0.0f);
+    const float M = wave_max(ml.x), f = ml.x == NINF ? 0.0f : __builtin_amdgcn_exp2f(ml.x - M), L = wave_sum(f * ml.y);
+    float acc[{N}];
     #pragma unroll
-    for (u32 i = 0; i < {(DP + 63) // 64}u; ++i) acc[i] = 0.0f;
+    for (u32 i = 0; i < {N}u; ++i) acc[i] = 0.0f;
+    #pragma unroll 8
     for (u32 s = 0; s < splits; ++s) {{
-        const float* __restrict__ ps = pr + s * (DP + 2u);
-        const float f = ps[DP] == NINF ? 0.0f : __builtin_amdgcn_exp2f(ps[DP] - M);
-        L += f * ps[DP + 1u];
+        const float fs = __shfl(f, (int)s, WAVE);
         #pragma unroll
-        for (u32 i = 0; i < {(DP + 63) // 64}u; ++i) {{ const u32 c = i * 64u + lane; if (c < d) acc[i] += f * ps[c]; }}
+        for (u32 i = 0; i < {N}u; ++i) {{ const u32 c = i * 64u + lane; if (c < d) acc[i] += fs * pr[s * (DP + 2u) + c]; }}
     }}
     float* __restrict__ yr = y + ((u64)b * T + row / group) * ((u64)H * group * d) + (u64)(h * group + row % group) * d;
+    const float inv = L == 0.0f ? 0.0f : 1.0f / L;
     #pragma unroll
-    for (u32 i = 0; i < {(DP + 63) // 64}u; ++i) {{ const u32 c = i * 64u + lane; if (c < d) yr[c] = L == 0.0f ? 0.0f : acc[i] / L; }}
+    for (u32 i = 0; i < {N}u; ++i) {{ const u32 c = i * 64u + lane; if (c < d) yr[c] = acc[i] * inv; }}
 }}
 """
     return src, name, _fmt("P" * 2, "I" * 6)

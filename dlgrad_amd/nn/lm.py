@@ -8,18 +8,24 @@ import math
 
 import numpy as np
 
+import dlgrad_amd.nn as _nn
 from dlgrad_amd import ops
-from dlgrad_amd.buffer import Buffer
+from dlgrad_amd.buffer import Buffer, HostScalar, _dispatch_table
 from dlgrad_amd.device import Device, as_device
-from dlgrad_amd.dispatch import dispatcher
 from dlgrad_amd.helpers import CustomOps
 from dlgrad_amd.tensor import Tensor
 
 
+def _result(buf: Buffer) -> Tensor:
+    """A tensor without a tape around a buffer (what Tensor(buf) makes)."""
+    t = Tensor.__new__(Tensor)
+    t.data, t.requires_grad, t._ctx, t.grad = buf, False, None, None
+    return t
+
+
 def _no_tape(what: str, *tensors) -> None:
     """Refuses a call whose result would silently stop a gradient."""
-    from dlgrad_amd import nn
-    if not nn._tape_free(*[t for t in tensors if isinstance(t, Tensor)]):
+    if any([t.requires_grad for t in tensors if t is not None]) and not _nn._inference_depth:
         raise ValueError(f"{what} has no gradient: call it inside nn.inference(), or with detach()ed tensors")
 
 
@@ -52,6 +58,10 @@ def rotary_frequencies(rotated: int, base: float = 10000.0, scaling: str | None 
     return f, 1.0
 
 
+def _on_hip(b: Buffer) -> bool:
+    return b.device is Device.HIP and b.ptr.__class__ is not HostScalar
+
+
 class Rotary:
     """Rotary positions for heads of `head_dim` elements, the first `rotated` of which turn (all by default):
 
@@ -71,7 +81,7 @@ class Rotary:
             raise ValueError(f"rotary: {rotated} of {head_dim} elements cannot turn")
         self.head_dim, self.rotated, self.half, self.device = head_dim, rotated, layout == "half", as_device(device)
         self.frequencies, self.gain = rotary_frequencies(rotated, base, scaling, factor, trained)
-        self._words = None
+        self._words, self._plans = None, {}
 
     def _table(self) -> Buffer:
         """The frequencies in turns per position as fractions of 2^64, on the device."""
@@ -90,22 +100,62 @@ class Rotary:
             raise ValueError(f"rotary: {x.shape} is neither (B, T, {n_head} * {self.head_dim}) nor (B, heads, T, {self.head_dim}) with n_head = 1")
         return x.numel // x.shape[-1] if x.shape[-1] else 0, x.shape[-2], x.shape[1] if x.ndim == 4 else 1
 
-    @staticmethod
-    def _given(t: Tensor | None) -> Buffer | None:
-        return None if t is None else t.data
-
     def __call__(self, x: Tensor, n_head: int = 1, positions: Tensor | None = None, start: Tensor | None = None, transpose: bool = False) -> Tensor:
         """x, (B, T, n_head * head_dim) or (B, heads, T, head_dim), turned by its positions: `positions` (T,) or (B, T), or 0 .. T - 1
         without them, plus `start` (one number, or one per sequence: a device tensor, so a captured step may move it).
         transpose: the transposed map, which turns the other way -- it takes a gradient of the result to one of x."""
-        return self._turn([x], [n_head], positions, start, transpose)[0]
+        xd, p, s0 = x.data, None if positions is None else positions.data, None if start is None else start.data
+        key = (xd.shape, n_head, None if p is None else p.shape, None if s0 is None else s0.shape, transpose)
+        plan = self._plans.get(key) if ops.FUSED and not x.requires_grad else None
+        if plan is None or not (_on_hip(xd) and (p is None or _on_hip(p)) and (s0 is None or _on_hip(s0))):
+            out = self._turn([x], [n_head], positions, start, transpose)
+            self._remember(key, [x], [n_head], p, s0, transpose)
+            return out[0]
+        return _result(xd._like(plan(xd.ptr, None, self._words.ptr.addr, 0 if p is None else p.ptr.addr, 0 if s0 is None else s0.ptr.addr)[0]))
 
     def pair(self, q: Tensor, k: Tensor, n_head: int, n_kv_head: int | None = None, positions: Tensor | None = None, start: Tensor | None = None,
              transpose: bool = False) -> tuple[Tensor, Tensor]:
         """(self(q), self(k)) with n_head and n_kv_head heads, in one launch on the hip device."""
-        return tuple(self._turn([q, k], [n_head, n_head if n_kv_head is None else n_kv_head], positions, start, transpose))
+        qd, kd = q.data, k.data
+        p, s0 = None if positions is None else positions.data, None if start is None else start.data
+        key = (qd.shape, kd.shape, n_head, n_kv_head, None if p is None else p.shape, None if s0 is None else s0.shape, transpose)
+        plan = self._plans.get(key) if ops.FUSED and not (q.requires_grad or k.requires_grad) else None
+        if plan is None or not (_on_hip(qd) and _on_hip(kd) and (p is None or _on_hip(p)) and (s0 is None or _on_hip(s0))):
+            heads = [n_head, n_head if n_kv_head is None else n_kv_head]
+            out = self._turn([q, k], heads, positions, start, transpose)
+            self._remember(key, [q, k], heads, p, s0, transpose)
+            return out[0], out[1]
+        y0, y1 = plan(qd.ptr, kd.ptr, self._words.ptr.addr, 0 if p is None else p.ptr.addr, 0 if s0 is None else s0.ptr.addr)
+        return _result(qd._like(y0)), _result(kd._like(y1))
+
+    def _remember(self, key: tuple, xs: list, heads: list, p: Buffer | None, s0: Buffer | None, back: bool) -> None:
+        """Keeps the launch of a call that has just passed its checks for calls of the same shapes."""
+        shapes = [self._geometry(x, h) for x, h in zip(xs, heads)]
+        if not ops.FUSED or not _on_hip(xs[0].data) or shapes[0][2] != shapes[-1][2] or key in self._plans:
+            return
+        from dlgrad_amd.runtime.hip_lm import HIPLM
+        if len(self._plans) >= 1024:                                   # (a workload whose shapes never repeat)
+            self._plans.clear()
+        plan = HIPLM.rotary_plan([(x.data.numel, h, h * self.head_dim) for x, h in zip(xs, heads)], self._words.numel, *shapes[0], self.head_dim,
+                                 self.rotated, self.half, bool(back), self.gain, 0 if p is None else p.numel, 0 if s0 is None else s0.numel, False)
+        if plan is not None:
+            self._plans[key] = plan
 
     def _turn(self, xs: list, heads: list, positions, start, back: bool) -> list:
+        shapes = self._check(xs, heads, positions, start)
+        if not ops.FUSED or xs[0].data.device is not Device.HIP:
+            return [self._composed(x, h, s, positions, start, back) for x, h, s in zip(xs, heads, shapes)]
+        back, p, s0 = bool(back), None if positions is None else positions.data, None if start is None else start.data
+        d = self.head_dim
+        if len(xs) == 1 or shapes[0][2] == shapes[1][2]:                # rows map to sequences alike: one launch
+            out = self._launch([(x.data, h, h * d) for x, h in zip(xs, heads)], shapes[0], back, p, s0)
+        else:
+            out = [self._launch([(x.data, h, h * d)], s, back, p, s0)[0] for x, h, s in zip(xs, heads, shapes)]
+        return [ops.Rotary.execute(x, turned=y, rope=self, n_head=h, geometry=s, positions=p, start=s0, back=back) if x.requires_grad else Tensor(y)
+                for x, y, h, s in zip(xs, out, heads, shapes)]
+
+    def _check(self, xs: list, heads: list, positions, start) -> list:
+        """Refuses shapes and devices that do not fit together; the geometry of each tensor."""
         shapes = [self._geometry(x, h) for x, h in zip(xs, heads)]
         x = xs[0]
         if any(t.device is not x.device for t in xs[1:] + [t for t in (positions, start) if t is not None]):
@@ -117,31 +167,23 @@ class Rotary:
             raise ValueError(f"rotary: positions {positions.shape} for {B} sequences of {T}")
         if start is not None and start.numel not in (1, B):
             raise ValueError(f"rotary: starts {start.shape} for {B} sequences")
-        if not ops.FUSED or x.device is not Device.HIP:
-            return [self._composed(x, h, s, positions, start, back) for x, h, s in zip(xs, heads, shapes)]
-        kw = dict(freq=self._table(), d=self.head_dim, rot=self.rotated, half=self.half, back=bool(back), gain=self.gain,
-                  positions=self._given(positions), start=self._given(start))
-        if len(xs) == 1 or shapes[0][2] == shapes[1][2]:                # rows map to sequences alike: one launch
-            rows, T, per = shapes[0]
-            out = Buffer.rotary([(x.data, h, h * self.head_dim) for x, h in zip(xs, heads)], rows=rows, T=T, per=per, **kw)
-        else:
-            out = [Buffer.rotary([(x.data, h, h * self.head_dim)], rows=s[0], T=s[1], per=s[2], **kw)[0] for x, h, s in zip(xs, heads, shapes)]
-        return [ops.Rotary.execute(x, turned=y, rope=self, n_head=h, geometry=s, positions=kw["positions"], start=kw["start"], back=bool(back))
-                for x, y, h, s in zip(xs, out, heads, shapes)]
+        return shapes
+
+    def _launch(self, parts: list, geometry: tuple, back: bool, positions: Buffer | None, start: Buffer | None, inplace: bool = False) -> list:
+        rows, T, per = geometry
+        return Buffer.rotary(parts, freq=self._words or self._table(), rows=rows, T=T, per=per, d=self.head_dim, rot=self.rotated, half=self.half,
+                             back=back, gain=self.gain, positions=positions, start=start, inplace=inplace)
 
     def turn_back(self, g: Buffer, n_head: int, geometry: tuple, positions: Buffer | None, start: Buffer | None, back: bool) -> Buffer:
         """The transposed map of a gradient."""
-        rows, T, per = geometry
-        return Buffer.rotary([(g, n_head, n_head * self.head_dim)], freq=self._table(), rows=rows, T=T, per=per, d=self.head_dim, rot=self.rotated,
-                             half=self.half, back=not back, gain=self.gain, positions=positions, start=start)[0]
+        return self._launch([(g, n_head, n_head * self.head_dim)], geometry, not back, positions, start)[0]
 
     def turn_qkv_(self, qkv: Buffer, n_head: int, back: bool = False) -> None:
         """In place, positions 0 .. T - 1: the query and key heads of a (B, T, 3 C) projection, C = n_head * head_dim."""
         B, T, C3 = qkv.shape
         if C3 != 3 * n_head * self.head_dim:
             raise ValueError(f"rotary: a projection {qkv.shape} for {n_head} heads of {self.head_dim}")
-        Buffer.rotary([(qkv, 2 * n_head, C3)], freq=self._table(), rows=B * T, T=T, per=1, d=self.head_dim, rot=self.rotated, half=self.half,
-                      back=back, gain=self.gain, inplace=True)
+        self._launch([(qkv, 2 * n_head, C3)], (B * T, T, 1), back, None, None, inplace=True)
 
     def _composed(self, x: Tensor, n_head: int, geometry: tuple, positions, start, back: bool) -> Tensor:
         """The same as x * cos + (x @ J) * sin with J the signed permutation that takes (a, b) of a pair to (-b, a): existing
@@ -204,7 +246,7 @@ class QuantizedKVCache:
         blocks = -(-capacity // self.BLOCK)
         self.capacity = blocks * self.BLOCK
         self.lengths = Tensor.full((batch, 1), 0.0, device="hip") if lengths is None else lengths
-        self.layers = [Cache8(batch, n_kv_head, head_dim, blocks) for _ in range(layers)]
+        self.layers = [Cache8(batch, n_kv_head, head_dim, blocks, layers) for _ in range(layers)]
 
     @property
     def nbytes(self) -> int:
@@ -213,30 +255,46 @@ class QuantizedKVCache:
     def _run(self, op, layer: int, counts: Tensor | None, **kw):
         if not 0 <= layer < len(self.layers):
             raise IndexError(f"layer {layer} of a cache of {len(self.layers)}")
-        if counts is not None and counts.__class__ is not Tensor:
-            raise TypeError("counts is a tensor with a number per sequence")
-        return dispatcher.dispatch(op=op, device=Device.HIP, cache=self.layers[layer], lengths=self.lengths.data,
-                                   counts=None if counts is None else counts.data, **kw)
+        if counts is not None:
+            if counts.__class__ is not Tensor:
+                raise TypeError("counts is a tensor with a number per sequence")
+            counts = counts.data
+        return _dispatch_table[(op, Device.HIP)](cache=self.layers[layer], lengths=self.lengths.data, counts=counts, **kw)
+
+    def _sized(self, counts: Tensor | None) -> bool:
+        """Whether the lengths and counts of a call are what the launch of an earlier call may read."""
+        n = self.lengths.data
+        return n.numel == self.batch and _on_hip(n) and (counts is None or (counts.__class__ is Tensor and counts.data.numel == self.batch and _on_hip(counts.data)))
 
     def write(self, k: Tensor, v: Tensor, layer: int = 0, counts: Tensor | None = None) -> None:
         """k, v (B, T, n_kv_head * head_dim): keys and values of positions lengths[b] .. of each sequence."""
         _no_tape("QuantizedKVCache.write", k, v)
-        self._run(CustomOps.CACHE8_WRITE, layer, counts, k=k.data, v=v.data)
+        kd, vd = k.data, v.data
+        run = self.layers[layer].writers.get(kd.shape) if 0 <= layer < len(self.layers) else None
+        if run is not None and kd.shape == vd.shape and _on_hip(kd) and _on_hip(vd) and self._sized(counts):
+            run(kd.ptr.addr, vd.ptr.addr, self.lengths.data.ptr.addr, 0 if counts is None else counts.data.ptr.addr)
+        else:
+            self._run(CustomOps.CACHE8_WRITE, layer, counts, k=kd, v=vd)
 
     def attend(self, q: Tensor, scale: float | None = None, layer: int = 0, counts: Tensor | None = None) -> Tensor:
         """q (B, T, n_head * head_dim): the queries of positions lengths[b] .., whose keys and values write() has stored; each sees
         the positions up to its own.  scale: of the scores, head_dim ** -0.5 without one."""
         _no_tape("QuantizedKVCache.attend", q)
         scale = self.head_dim ** -0.5 if scale is None else float(scale)
-        y = self._run(CustomOps.CACHE8_ATTEND, layer, counts, q=q.data, scale=scale)
-        return Tensor(Buffer.fresh(y, q.shape, Device.HIP), requires_grad=False)
+        qd = q.data
+        run = self.layers[layer].attenders.get(qd.shape) if 0 <= layer < len(self.layers) else None
+        if run is not None and _on_hip(qd) and self._sized(counts):
+            y = run(qd.ptr.addr, self.lengths.data.ptr.addr, 0 if counts is None else counts.data.ptr.addr, scale)
+        else:
+            y = self._run(CustomOps.CACHE8_ATTEND, layer, counts, q=qd, scale=scale)
+        return _result(Buffer.fresh(y, qd.shape, Device.HIP))
 
     def read(self, n: int, layer: int = 0, new: int = 0, counts: Tensor | None = None) -> tuple[Tensor, Tensor]:
         """(k, v), both (B, n, n_kv_head * head_dim): the values that the first n positions stand for, zeros where a sequence is
         shorter.  new, or counts: rows that were written since the last advance() and belong to it."""
         k, v = self._run(CustomOps.CACHE8_READ, layer, counts, n=int(n), extra=self.capacity if counts is not None else int(new))
         shape = (self.batch, int(n), self.n_kv_head * self.head_dim)
-        return tuple(Tensor(Buffer.fresh(t, shape, Device.HIP), requires_grad=False) for t in (k, v))
+        return _result(Buffer.fresh(k, shape, Device.HIP)), _result(Buffer.fresh(v, shape, Device.HIP))
 
     def advance(self, n: "int | Tensor") -> None:
         """The rows written become part of the sequences: n of each, or n (B, 1) of them."""
@@ -255,17 +313,10 @@ class QuantizedKVCache:
         self.lengths.data.copy_(Tensor.full(self.lengths.shape, 0.0, device="hip").data)
 
 
-def adjust_logits(logits: Tensor, history: Tensor | None = None, lengths: Tensor | None = None, repetition: "float | Tensor" = 1.0,
-                  presence: "float | Tensor" = 0.0, frequency: "float | Tensor" = 0.0, bias: Tensor | None = None,
-                  hidden: Tensor | None = None) -> Tensor:
-    """logits (B, V) before a token is chosen from them (decode_append, decode_sample, argmax): a new tensor without a tape.
+_adjust_plans: dict = {}       # shapes and numbers that _check_adjust has let through -> the launch (False off the hip device)
 
-    history (B, L): token ids said so far, the first lengths[b] of each row (all without lengths); ids outside [0, V) count for
-    nothing.  A token that occurs c > 0 times there becomes x / repetition if x > 0 and x * repetition otherwise, less
-    presence + frequency * c; the three are numbers, or tensors with one per row.  Then bias (V,) or (B, V) is added, and
-    tokens that hidden (V,) or (B, V) marks (> 0: a grammar's mask) become -inf whatever they were; a row may be hidden
-    whole.  One launch on the hip device; elsewhere on the host, from the downloaded logits."""
-    _no_tape("adjust_logits", logits, bias)
+
+def _check_adjust(logits, history, lengths, repetition, presence, frequency, bias, hidden) -> None:
     if logits.ndim != 2:
         raise ValueError(f"adjust_logits: logits {logits.shape} are not (B, V)")
     for name, p in (("repetition", repetition), ("presence", presence), ("frequency", frequency)):
@@ -285,11 +336,36 @@ def adjust_logits(logits: Tensor, history: Tensor | None = None, lengths: Tensor
     for name, p in (("repetition", repetition), ("presence", presence), ("frequency", frequency)):
         if isinstance(p, Tensor) and p.numel != B:
             raise ValueError(f"adjust_logits: {p.numel} values of {name} for {B} rows")
-    data = lambda t: t.data if isinstance(t, Tensor) else t              # noqa: E731
-    if ops.FUSED and logits.device is Device.HIP:
-        y = logits.data.adjust_logits(data(history), data(lengths), tuple(data(p) for p in (repetition, presence, frequency)), data(bias), data(hidden))
-        return Tensor(y, requires_grad=False)
-    x = logits.numpy().astype(np.float32, copy=True)
+
+
+def adjust_logits(logits: Tensor, history: Tensor | None = None, lengths: Tensor | None = None, repetition: "float | Tensor" = 1.0,
+                  presence: "float | Tensor" = 0.0, frequency: "float | Tensor" = 0.0, bias: Tensor | None = None,
+                  hidden: Tensor | None = None) -> Tensor:
+    """logits (B, V) before a token is chosen from them (decode_append, decode_sample, argmax): a new tensor without a tape.
+
+    history (B, L): token ids said so far, the first lengths[b] of each row (all without lengths); ids outside [0, V) count for
+    nothing.  A token that occurs c > 0 times there becomes x / repetition if x > 0 and x * repetition otherwise, less
+    presence + frequency * c; the three are numbers, or tensors with one per row.  Then bias (V,) or (B, V) is added, and
+    tokens that hidden (V,) or (B, V) marks (> 0: a grammar's mask) become -inf whatever they were; a row may be hidden
+    whole.  One launch on the hip device; elsewhere on the host, from the downloaded logits."""
+    _no_tape("adjust_logits", logits, bias)
+    given = (logits, history, lengths, repetition, presence, frequency, bias, hidden)
+    key = tuple([(t.data.shape, t.data.device, t.data.ptr.__class__) if t.__class__ is Tensor else t for t in given])
+    plan = _adjust_plans.get(key)
+    if plan is None:
+        _check_adjust(*given)
+        args = [t.data if isinstance(t, Tensor) else t for t in given]
+        plan = False                                                    # (checked; not launched from here)
+        if logits.data.device is Device.HIP:
+            from dlgrad_amd.runtime.hip_lm import HIPLM
+            plan = HIPLM.logits_plan(*args[:3], tuple(args[3:6]), *args[6:])
+        if len(_adjust_plans) >= 1024:                                  # (a workload whose shapes never repeat)
+            _adjust_plans.clear()
+        _adjust_plans[key] = plan
+    if plan and ops.FUSED:
+        x, h, n, r, p, f, b, m = [t.data if t.__class__ is Tensor else t for t in given]
+        return _result(x._like(plan(x, h, n, (r, p, f), b, m)))
+    (B, V), x = logits.shape, logits.numpy().astype(np.float32, copy=True)
     rows = lambda p: p.numpy().reshape(B) if isinstance(p, Tensor) else np.full(B, p, np.float32)      # noqa: E731
     rep, pre, fre = rows(repetition), rows(presence), rows(frequency)
     if history is not None and history.shape[1]:

@@ -3,6 +3,8 @@ and the adjustment of logits.  Checks of shapes and addresses, choice of the ker
 kernels are in codegen/lm_kernel.py."""
 from __future__ import annotations
 
+import math
+
 import numpy as np
 
 from dlgrad_amd.buffer import Buffer
@@ -10,9 +12,11 @@ from dlgrad_amd.codegen import lm_kernel as K
 from dlgrad_amd.device import Device
 from dlgrad_amd.dispatch import dispatcher
 from dlgrad_amd.helpers import CustomOps
-from dlgrad_amd.runtime.hip import DevicePtr, _addr, _upload, alloc, kernel, launch, props
+from dlgrad_amd.runtime.hip import DevicePtr, _addr, _PlanCache, _upload, alloc, field_offset, kernel, launch, launch_out, props
 
+STREAM_BYTES = 1 << 28       # the Infinity Cache
 EXACT_WHOLE = 1 << 24        # whole numbers up to here are exact in fp32
+_rotary_plans: dict = _PlanCache()     # what a call looked at -> the launch that its checks ended in
 
 
 def _on_device(what: str, **tensors) -> None:
@@ -21,17 +25,15 @@ def _on_device(what: str, **tensors) -> None:
             raise ValueError(f"{what}: {name} is not a tensor on the hip device")
 
 
-def _aligned(*addrs: int) -> bool:
-    return not any(a & 15 for a in addrs)
-
-
 class Cache8:
     """One layer of an 8-bit key/value cache in device memory: codes, scales and the fp32 tails."""
-    __slots__ = ("batch", "heads", "d", "width", "blocks", "kc", "vc", "scales", "tail_k", "tail_v")
+    __slots__ = ("batch", "heads", "d", "width", "blocks", "layers", "kc", "vc", "scales", "tail_k", "tail_v", "writers", "attenders")
 
-    def __init__(self, batch: int, heads: int, d: int, blocks: int) -> None:
-        self.batch, self.heads, self.d, self.blocks = batch, heads, d, blocks
+    def __init__(self, batch: int, heads: int, d: int, blocks: int, layers: int = 1) -> None:
+        """layers: how many of these a step reads one after the other."""
+        self.batch, self.heads, self.d, self.blocks, self.layers = batch, heads, d, blocks, layers
         self.width = K.cache8_width(d)
+        self.writers, self.attenders = _PlanCache(), _PlanCache()            # shape of a call -> the launch that its checks ended in
         n = batch * heads * blocks
         codes = n * K.CACHE8_BLOCK * self.width // 4                       # in units of 4 bytes, as everything is allocated
         self.kc, self.vc = alloc(codes), alloc(codes)                        # (a block is written whole before its first read)
@@ -47,9 +49,6 @@ class Cache8:
 class HIPLM:
     """Dispatch-table entries for Device.HIP."""
 
-    # workgroups the 8-bit attention aims for when it splits the tokens of a sequence
-    ATTEND_WORKGROUPS_PER_CU = 4
-
     @staticmethod
     def words(a: np.ndarray) -> Buffer:
         """A host array of 64-bit words in device memory, as a Buffer of twice as many floats that nothing does arithmetic on."""
@@ -60,47 +59,84 @@ class HIPLM:
 
     # ---- rotary positions ------------------------------------------------------------------------
     @staticmethod
-    @dispatcher.register(CustomOps.ROTARY, Device.HIP)
-    def rotary(parts: list, freq: Buffer, rows: int, T: int, per: int, d: int, rot: int, half: bool, back: bool, gain: float,
-               positions: Buffer | None = None, start: Buffer | None = None, inplace: bool = False) -> list:
-        """parts: one or two (Buffer, heads, pitch): `rows` rows of `heads` heads of d, `pitch` floats apart.  Row i is position
-        i % T of sequence i // T // per.  Returns the turned tensors' pointers (rows * heads * d floats each), or writes
-        the parts themselves when `inplace`."""
-        _on_device("rotary", positions=positions, start=start, **{f"x{i}": p[0] for i, p in enumerate(parts)})
-        if not 1 <= len(parts) <= 2 or not 0 < rot <= d or rot % 2 or freq.numel != rot:
-            raise ValueError(f"rotary: {len(parts)} tensors, {rot} of {d} elements turned, {freq.numel // 2} frequencies")
+    def rotary_plan(sizes: list, n_words: int, rows: int, T: int, per: int, d: int, rot: int, half: bool, back: bool, gain: float,
+                    n_positions: int, n_starts: int, inplace: bool):
+        """The checks of a call that depend on sizes alone, and the launch of everything else.  sizes: one or two (elements, heads,
+        pitch): `rows` rows of `heads` heads of d, `pitch` floats apart.  Row i is position i % T of sequence i // T // per.
+        Returns run(pointer, second pointer, addresses of the frequencies, the positions and the starts) -> two pointers, or None where there
+        is nothing to do."""
+        if not 1 <= len(sizes) <= 2 or not 0 < rot <= d or rot % 2 or n_words != rot:
+            raise ValueError(f"rotary: {len(sizes)} tensors, {rot} of {d} elements turned, {n_words // 2} frequencies")
         if rows == 0:
-            return [x.ptr if inplace else alloc(0) for x, _, _ in parts]
+            return None
         if T < 1 or per < 1 or rows % (T * per) or T > EXACT_WHOLE:
             raise ValueError(f"rotary: {rows} rows are not whole sequences of {T}")
         batch = rows // (T * per)
-        for x, heads, pitch in parts:
-            if heads < 1 or pitch < heads * d or x.numel < (rows - 1) * pitch + heads * d:
-                raise ValueError(f"rotary: {rows} rows of {heads} heads of {d} are not in a tensor of {x.numel} elements with rows {pitch} apart")
+        for numel, heads, pitch in sizes:
+            if heads < 1 or pitch < heads * d or numel < (rows - 1) * pitch + heads * d:
+                raise ValueError(f"rotary: {rows} rows of {heads} heads of {d} are not in a tensor of {numel} elements with rows {pitch} apart")
             if pitch >= 2 ** 32:
                 raise ValueError(f"rotary: rows {pitch} elements apart exceed the kernel's 32-bit pitch")
-        if positions is not None and positions.numel not in (T, batch * T):
-            raise ValueError(f"rotary: {positions.numel} positions for {batch} sequences of {T}")
-        if start is not None and start.numel not in (1, batch):
-            raise ValueError(f"rotary: {start.numel} starts for {batch} sequences")
-        outs = [x.ptr if inplace else alloc(rows * heads * d) for x, heads, _ in parts]
-        out_pitch = [p if inplace else h * d for _, h, p in parts]
-        addrs = [_addr(x) for x, _, _ in parts]
+        if n_positions not in (0, T, batch * T):
+            raise ValueError(f"rotary: {n_positions} positions for {batch} sequences of {T}")
+        if n_starts not in (0, 1, batch):
+            raise ValueError(f"rotary: {n_starts} starts for {batch} sequences")
+        two = len(sizes) - 1
+        out_pitch = [p if inplace else h * d for _, h, p in sizes]
         unit = 8 if half else 4                                        # elements of a unit of pairs in 16-byte accesses
-        vec = rot % unit == 0 and d % 4 == 0 and all(p % 4 == 0 for _, _, p in parts) and _aligned(*addrs, *[o.addr for o in outs])
-        units = rot // unit if vec else rot // 2
-        if not inplace:
-            units += (d - rot) // (4 if vec else 1)
-        most = max(rows * -(-h // K.ROTARY_HEADS) * units for _, h, _ in parts)
-        if (most + 255) // 256 >= 2 ** 31:
-            raise ValueError(f"rotary: {rows} rows exceed the grid")
-        two = len(parts) - 1
-        launch(kernel(K.rotary_kernel, half, vec), ((most + 255) // 256, 1, 1 + two), 256, addrs[0], outs[0].addr, addrs[two], outs[two].addr,
-               _addr(freq), _addr(positions) if positions is not None else 0, _addr(start) if start is not None else 0,
-               rows, T, per, parts[0][1], parts[two][1], d, rot, parts[0][2], parts[two][2], out_pitch[0], out_pitch[two],
-               T if positions is not None and positions.numel == batch * T else 0,
-               1 if start is not None and start.numel == batch else 0, int(back), float(gain))
-        return outs
+        wide = rot % unit == 0 and d % 4 == 0 and all(p % 4 == 0 for _, _, p in sizes)
+
+        def grid(vec: bool) -> tuple:
+            units = (rot // unit if vec else rot // 2) + (0 if inplace else (d - rot) // (4 if vec else 1))
+            blocks = (max(rows * -(-h // K.ROTARY_HEADS) * units for _, h, _ in sizes) + 255) // 256
+            if blocks >= 2 ** 31:
+                raise ValueError(f"rotary: {rows} rows exceed the grid")
+            return (blocks, 1, 1 + two)
+
+        def variant(vec: bool) -> list:
+            v = [None, grid(vec), None]
+
+            def load():
+                v[0] = kernel(K.rotary_kernel, half, vec)
+                return v[0]
+            v[2] = load
+            return v
+        narrow = variant(False)
+        first = variant(True) if wide else narrow
+        tail = (rows, T, per, sizes[0][1], sizes[two][1], d, rot, sizes[0][2], sizes[two][2], out_pitch[0], out_pitch[two],
+                T if n_positions == batch * T else 0, 1 if n_starts == batch else 0, int(back), float(gain))
+        numel0, numel1 = rows * sizes[0][1] * d, rows * sizes[two][1] * d
+
+        def run(x0: DevicePtr, x1: DevicePtr | None, table: int, pos: int, start: int) -> tuple:
+            a0 = x0.addr
+            a1 = x1.addr if two else a0
+            y0 = x0 if inplace else alloc(numel0)
+            y1 = y0 if not two else x1 if inplace else alloc(numel1)
+            v = narrow if (a0 | a1) & 15 else first                  # (fresh blocks are aligned)
+            k = v[0] or v[2]()
+            launch(k, v[1], 256, a0, y0.addr, a1, y1.addr, table, pos, start, *tail)
+            return y0, y1
+        return run
+
+    @staticmethod
+    @dispatcher.register(CustomOps.ROTARY, Device.HIP)
+    def rotary(parts: list, freq: Buffer, rows: int, T: int, per: int, d: int, rot: int, half: bool, back: bool, gain: float,
+               positions: Buffer | None = None, start: Buffer | None = None, inplace: bool = False) -> list:
+        """parts: one or two (Buffer, heads, pitch), see rotary_plan.  Returns the turned tensors' pointers (rows * heads * d floats
+        each), or writes the parts themselves when `inplace`."""
+        bufs = [p[0] for p in parts]
+        key = (freq.numel, rows, T, per, d, rot, half, back, gain, inplace, *[(b.numel, h, p, b.device, b.ptr.__class__) for b, h, p in parts],
+               None if positions is None else (positions.numel, positions.device, positions.ptr.__class__),
+               None if start is None else (start.numel, start.device, start.ptr.__class__))
+        plan = _rotary_plans.get(key, _rotary_plans)
+        if plan is _rotary_plans:
+            _on_device("rotary", positions=positions, start=start, **{f"x{i}": b for i, b in enumerate(bufs)})
+            plan = _rotary_plans[key] = HIPLM.rotary_plan([(b.numel, h, p) for b, h, p in parts], freq.numel, rows, T, per, d, rot, half, back, gain,
+                                                          0 if positions is None else positions.numel, 0 if start is None else start.numel, inplace)
+        if plan is None:
+            return [b.ptr if inplace else alloc(0) for b in bufs]
+        return plan(bufs[0].ptr, bufs[-1].ptr, freq.ptr.addr, positions.ptr.addr if positions is not None else 0,
+                    start.ptr.addr if start is not None else 0)[:len(parts)]
 
     # ---- the 8-bit cache ---------------------------------------------------------------------------
     @staticmethod
@@ -110,58 +146,124 @@ class HIPLM:
             raise ValueError(f"{what}: {lengths.numel} lengths and {'no' if counts is None else counts.numel} counts for {c.batch} sequences")
 
     @staticmethod
-    @dispatcher.register(CustomOps.CACHE8_WRITE, Device.HIP)
-    def cache8_write(cache: Cache8, k: Buffer, v: Buffer, lengths: Buffer, counts: Buffer | None = None) -> None:
-        c = cache
-        _on_device("cache8_write", k=k, v=v)
-        HIPLM._cache8_lengths("cache8_write", c, lengths, counts)
-        C = c.heads * c.d
-        if k.ndim != 3 or k.shape != v.shape or k.shape[0] != c.batch or k.shape[2] != C:
-            raise ValueError(f"cache8_write: keys {k.shape} and values {v.shape} for {c.batch} sequences of {c.heads} heads of {c.d}")
-        T = k.shape[1]
-        if T > c.blocks * K.CACHE8_BLOCK:
-            raise ValueError(f"cache8_write: {T} tokens for a cache of {c.blocks * K.CACHE8_BLOCK}")
-        if T == 0:
-            return
-        vec = C % 4 == 0 and c.d % 4 == 0 and _aligned(_addr(k), _addr(v))
-        # a call may complete the block it starts in and ceil(T / 64) more
-        launch(kernel(K.cache8_write_kernel, c.width, vec), (1 + -(-T // K.CACHE8_BLOCK), c.heads, c.batch), 256, _addr(k), _addr(v),
-               _addr(lengths), _addr(counts) if counts is not None else 0, c.kc.addr, c.vc.addr, _addr(c.scales), _addr(c.tail_k), _addr(c.tail_v),
-               T, c.heads, c.d, c.blocks, C, C)
+    def write_threads(workgroups: int, compute_units: int) -> int:
+        """Threads per block of 64 tokens that the write takes.  A launch of few workgroups is one pass over the code, shorter with fewer
+        elements a thread (1 x 8 heads of 128, 512 tokens: 12.1 us with 256, 8.3 with 512, 7.2 with 1024); many small ones hide
+        each other's barriers (8 x 12 heads of 64, 1024 tokens: 20.4, 17.5, 20.4 us; 4 x 12 x 4096: 37.2, 32.5, 40.7)."""
+        return 1024 if workgroups <= 2 * compute_units else 512
 
     @staticmethod
-    def attend_splits(groups: int, blocks: int, compute_units: int) -> int:
-        """Into how many parts the blocks of a sequence are cut when one part makes `groups` workgroups: enough to fill the
-        device, and four blocks a part at least, one for each wavefront.  The length is device data, so the capacity
-        stands for it; a part whose blocks are not there yet costs its launch."""
-        return max(1, min(HIPLM.ATTEND_WORKGROUPS_PER_CU * compute_units // max(groups, 1), (blocks + 3) // 4))
+    def cache8_writer(c: Cache8, shape: tuple):
+        """The checks of cache8_write that depend on the shape of the keys alone, and run(addresses of keys, values, lengths, counts)."""
+        C = c.heads * c.d
+        if len(shape) != 3 or shape[0] != c.batch or shape[2] != C:
+            raise ValueError(f"cache8_write: keys {shape} for {c.batch} sequences of {c.heads} heads of {c.d}")
+        T = shape[1]
+        if T > c.blocks * K.CACHE8_BLOCK:
+            raise ValueError(f"cache8_write: {T} tokens for a cache of {c.blocks * K.CACHE8_BLOCK}")
+        NT = HIPLM.write_threads(-(-T // K.CACHE8_BLOCK) * c.heads * c.batch, props()["compute_units"])
+        grid, wide, kernels = (-(-T // K.CACHE8_BLOCK), c.heads, c.batch), C % 4 == 0 and c.d % 4 == 0, [None, None]
+        tail = (c.kc.addr, c.vc.addr, _addr(c.scales), _addr(c.tail_k), _addr(c.tail_v), T, c.heads, c.d, c.blocks, C, C)
+
+        def run(ka: int, va: int, la: int, ca: int) -> None:
+            vec = wide and not (ka | va) & 15
+            k = kernels[vec]
+            if k is None:
+                k = kernels[vec] = kernel(K.cache8_write_kernel, c.width, vec, NT)
+            # a call completes at most ceil(T / 64) blocks, the one it starts in among them
+            launch(k, grid, NT, ka, va, la, ca, *tail)
+        return run if T else lambda ka, va, la, ca: None
+
+    @staticmethod
+    @dispatcher.register(CustomOps.CACHE8_WRITE, Device.HIP)
+    def cache8_write(cache: Cache8, k: Buffer, v: Buffer, lengths: Buffer, counts: Buffer | None = None) -> None:
+        _on_device("cache8_write", k=k, v=v)
+        HIPLM._cache8_lengths("cache8_write", cache, lengths, counts)
+        if v.shape != k.shape:
+            raise ValueError(f"cache8_write: keys {k.shape} and values {v.shape}")
+        run = cache.writers.get(k.shape)
+        if run is None:
+            run = cache.writers[k.shape] = HIPLM.cache8_writer(cache, k.shape)
+        run(_addr(k), _addr(v), _addr(lengths), 0 if counts is None else _addr(counts))
+
+    @staticmethod
+    def attend_tiles(rows: int, pairs: int, width: int, compute_units: int) -> int:
+        """Tiles of 16 query rows that a wavefront of the 8-bit attention holds.  Two share the widening of the codes (4 x 12 heads of 64,
+        512 rows after 4096 tokens: 77 us against 85; 8 x 12 heads, 1024 after 1024: 129 against 135) but halve the
+        workgroups, of which there should be three for every compute unit (the same with 256 rows: 53 us against 50); heads wider
+        than 64 have no registers for them (2 x 8 heads of 128, 512 after 2048: 40.6 us both ways)."""
+        return 2 if width <= 64 and pairs * -(-rows // 32) >= 3 * compute_units else 1
+
+    @staticmethod
+    def attend_waves(tiles: int, blocks: int, width: int) -> int:
+        """Wavefronts of a workgroup of the 8-bit attention.  With one tile of query rows, eight halve the blocks that each goes through
+        (16 x 12 heads of 64 over 4096 tokens: 19.1 us against 23.1 with four); heads wider than 64 fill the registers with four
+        (4 x 8 heads of 128 over 8192: 22.5 us, 23.0 with eight), and so few blocks as four leave the others idle (5.7, 6.3 us)."""
+        return 8 if tiles == 1 and width <= 64 and blocks > 4 else 4
+
+    @staticmethod
+    def attend_streams(c: Cache8, tiles: int) -> bool:
+        """Whether the codes bypass the caches: they are read once by a call, and the cache as a whole, all layers of it, is larger than
+        the 256 MiB that a later step might find them in (16 x 8 heads of 128 over 32768 tokens, 1.07 GB: 171 us against 192;
+        16 x 12 heads of 64 over 8192, 0.2 GB, again and again: 43.0 us against 38.4)."""
+        return tiles == 1 and c.layers * (c.kc.nbytes + c.vc.nbytes) > STREAM_BYTES
+
+    @staticmethod
+    def attend_splits(groups: int, blocks: int, waves: int, compute_units: int) -> int:
+        """Into how many parts the blocks of a sequence are cut when one part makes `groups` workgroups of `waves` wavefronts.  A wavefront
+        takes 0.8 us for a block when there are few, the second launch that joins the parts 3.5 us and 0.1 us for each:
+        sqrt(blocks / 2) parts from 8 blocks a wavefront on (1 x 12 heads of 64 over 4096 tokens, four wavefronts: 18.0 us
+        with one part, 11.9 with 4, 12.0 with 16; 1 x 8 heads of 128 over 32768: 40 us with 8, 34 with 16, 37 with 32), and no more than
+        eight wavefronts for every compute unit (16 x 12 heads of 64 over 4096: 23.4 us with 2 parts, 27.1 with 8).  The length is
+        device data; the capacity stands for it."""
+        if blocks < 8 * waves:
+            return 1
+        return max(1, min(8 * compute_units // (waves * max(groups, 1)), math.isqrt(blocks // 2), K.CACHE8_MAX_SPLITS))
+
+    @staticmethod
+    def cache8_attender(c: Cache8, shape: tuple):
+        """The checks of cache8_attend that depend on the shape of the queries alone, and run(addresses of queries, lengths, counts,
+        scale) -> pointer."""
+        if len(shape) != 3 or shape[0] != c.batch or shape[2] == 0 or shape[2] % (c.heads * c.d):
+            raise ValueError(f"cache8_attend: queries {shape} for {c.batch} sequences with {c.heads} key heads of {c.d}")
+        T, group = shape[1], shape[2] // (c.heads * c.d)
+        if T > c.blocks * K.CACHE8_BLOCK:
+            raise ValueError(f"cache8_attend: {T} positions for a cache of {c.blocks * K.CACHE8_BLOCK}")
+        rows, pairs, numel = T * group, c.batch * c.heads, shape[0] * T * shape[2]
+        if not rows:
+            return lambda qa, la, ca, scale: alloc(0)
+        nq = HIPLM.attend_tiles(rows, pairs, c.width, props()["compute_units"])
+        tiles = -(-rows // (16 * nq))
+        waves = HIPLM.attend_waves(tiles, c.blocks, c.width)
+        splits = HIPLM.attend_splits(pairs * tiles, c.blocks, waves, props()["compute_units"])
+        grid = pairs * tiles * splits
+        if grid >= 2 ** 31 or pairs * rows >= 2 ** 31:
+            raise ValueError(f"cache8_attend: {pairs} heads of {rows} query rows exceed the grid")
+        k, join = kernel(K.cache8_attend_kernel, c.width, nq, waves, HIPLM.attend_streams(c, tiles)), kernel(K.cache8_join_kernel, c.width) if splits > 1 else None
+        held = (c.kc.addr, c.vc.addr, _addr(c.scales), _addr(c.tail_k), _addr(c.tail_v))
+        sizes = (c.batch, T, c.heads, group, c.d, c.blocks, tiles, splits)
+        n_part, join_grid, join_sizes = pairs * rows * splits * (c.width + 2), (pairs * rows + 3) // 4, (pairs * rows, T, c.heads, group, c.d, splits)
+
+        def run(qa: int, la: int, ca: int, scale: float) -> DevicePtr:
+            y = alloc(numel)
+            if join is None:
+                launch(k, grid, 64 * waves, qa, *held, la, ca, y.addr, 0, *sizes, scale)
+                return y
+            part = alloc(n_part)
+            launch(k, grid, 64 * waves, qa, *held, la, ca, y.addr, part.addr, *sizes, scale)
+            launch(join, join_grid, 256, part.addr, y.addr, *join_sizes)
+            return y
+        return run
 
     @staticmethod
     @dispatcher.register(CustomOps.CACHE8_ATTEND, Device.HIP)
     def cache8_attend(cache: Cache8, q: Buffer, scale: float, lengths: Buffer, counts: Buffer | None = None) -> DevicePtr:
-        c = cache
         _on_device("cache8_attend", q=q)
-        HIPLM._cache8_lengths("cache8_attend", c, lengths, counts)
-        if q.ndim != 3 or q.shape[0] != c.batch or q.shape[2] == 0 or q.shape[2] % (c.heads * c.d):
-            raise ValueError(f"cache8_attend: queries {q.shape} for {c.batch} sequences with {c.heads} key heads of {c.d}")
-        T, group = q.shape[1], q.shape[2] // (c.heads * c.d)
-        if T > c.blocks * K.CACHE8_BLOCK:
-            raise ValueError(f"cache8_attend: {T} positions for a cache of {c.blocks * K.CACHE8_BLOCK}")
-        y = alloc(q.numel)
-        if q.numel == 0:
-            return y
-        rows, pairs = T * group, c.batch * c.heads
-        tiles = -(-rows // 16)
-        splits = HIPLM.attend_splits(pairs * tiles, c.blocks, props()["compute_units"])
-        if pairs * tiles * splits >= 2 ** 31 or pairs * rows >= 2 ** 31:
-            raise ValueError(f"cache8_attend: {pairs} heads of {rows} query rows exceed the grid")
-        part = alloc(pairs * rows * splits * (c.width + 2)) if splits > 1 else None
-        launch(kernel(K.cache8_attend_kernel, c.width), pairs * tiles * splits, 256, _addr(q), c.kc.addr, c.vc.addr, _addr(c.scales), _addr(c.tail_k),
-               _addr(c.tail_v), _addr(lengths), _addr(counts) if counts is not None else 0, y.addr, part.addr if part is not None else 0,
-               c.batch, T, c.heads, group, c.d, c.blocks, tiles, splits, float(scale))
-        if part is not None:
-            launch(kernel(K.cache8_join_kernel, c.width), (pairs * rows + 3) // 4, 256, part.addr, y.addr, pairs * rows, T, c.heads, group, c.d, splits)
-        return y
+        HIPLM._cache8_lengths("cache8_attend", cache, lengths, counts)
+        run = cache.attenders.get(q.shape)
+        if run is None:
+            run = cache.attenders[q.shape] = HIPLM.cache8_attender(cache, q.shape)
+        return run(_addr(q), _addr(lengths), 0 if counts is None else _addr(counts), float(scale))
 
     @staticmethod
     @dispatcher.register(CustomOps.CACHE8_READ, Device.HIP)
@@ -193,6 +295,11 @@ class HIPLM:
     def adjust_logits(logits: Buffer, history: Buffer | None, lengths: Buffer | None, penalties: tuple, bias: Buffer | None, hidden: Buffer | None) -> DevicePtr:
         """logits (B, V); history (B, L); lengths B; penalties: (repetition, presence, frequency), each a float or a Buffer of B;
         bias and hidden: V or (B, V)."""
+        return HIPLM.logits_plan(logits, history, lengths, penalties, bias, hidden)(logits, history, lengths, penalties, bias, hidden)
+
+    @staticmethod
+    def logits_plan(logits: Buffer, history: Buffer | None, lengths: Buffer | None, penalties: tuple, bias: Buffer | None, hidden: Buffer | None):
+        """The checks of a call, which depend on shapes alone, and run(the same arguments) -> pointer for every call that agrees in them."""
         pen = [p if isinstance(p, Buffer) else None for p in penalties]
         _on_device("adjust_logits", logits=logits, history=history, lengths=lengths, bias=bias, hidden=hidden, repetition=pen[0], presence=pen[1], frequency=pen[2])
         if logits.ndim != 2 or logits.shape[1] > EXACT_WHOLE:
@@ -208,16 +315,29 @@ class HIPLM:
         for name, p in zip(("repetition", "presence", "frequency"), pen):
             if p is not None and p.numel != B:
                 raise ValueError(f"adjust_logits: {p.numel} values of {name} for {B} rows")
-        y = alloc(B * V)
-        if B * V == 0:
-            return y
         if B > 65535:
             raise ValueError(f"adjust_logits: {B} rows, at most 65535 in one call")
-        addr = lambda t: 0 if t is None else _addr(t)                     # noqa: E731
-        vec = V % 4 == 0 and _aligned(_addr(logits), addr(bias), addr(hidden), y.addr)
         items = HIPLM.adjust_items(B, V, props()["compute_units"])
-        launch(kernel(K.adjust_logits_kernel, items, vec), (-(-V // (256 * items)), B, 1), 256, _addr(logits), addr(history), addr(lengths),
-               addr(bias), addr(hidden), y.addr, *[addr(p) for p in pen], V, 0 if history is None else history.shape[1],
-               V if bias is not None and bias.numel == B * V else 0, V if hidden is not None and hidden.numel == B * V else 0,
-               *[0.0 if isinstance(p, Buffer) else float(p) for p in penalties])
-        return y
+        if B * V == 0:
+            return lambda *given: alloc(0)
+        wide, grid, kernels, out_at = V % 4 == 0, (-(-V // (256 * items)), B, 1), [None, None], field_offset("@" + "P" * 6, 5)
+        sizes = (V, 0 if history is None else history.shape[1], V if bias is not None and bias.numel == B * V else 0,
+                 V if hidden is not None and hidden.numel == B * V else 0)
+
+        def run(logits, history, lengths, penalties, bias, hidden) -> DevicePtr:
+            la, ba, ha = logits.ptr.addr, 0 if bias is None else bias.ptr.addr, 0 if hidden is None else hidden.ptr.addr
+            vec = wide and not (la | ba | ha) & 15
+            k = kernels[vec]
+            if k is None:
+                k = kernels[vec] = kernel(K.adjust_logits_kernel, items, vec, sizes[1] <= K.LOGITS_PACKED_L)
+            r, p, f = penalties
+            ra = pa = fa = 0
+            if isinstance(r, Buffer):
+                ra, r = r.ptr.addr, 1.0
+            if isinstance(p, Buffer):
+                pa, p = p.ptr.addr, 0.0
+            if isinstance(f, Buffer):
+                fa, f = f.ptr.addr, 0.0
+            return launch_out(k, grid, 256, out_at, B * V, la, 0 if history is None else history.ptr.addr, 0 if lengths is None else lengths.ptr.addr,
+                              ba, ha, 0, ra, pa, fa, *sizes, r, p, f)
+        return run

@@ -29,10 +29,12 @@ def within(got, want, tol, what=""):
         return
     got, want = np.asarray(got, np.float64), np.asarray(want, np.float64)
     assert got.shape == want.shape, f"{what}: {got.shape} vs {want.shape}"
+    if not want.size:
+        return
     odd = ~np.isfinite(want)
     np.testing.assert_array_equal(got[odd], want[odd], err_msg=what)
     assert np.isfinite(got[~odd]).all(), f"{what}: not finite where it should be"
-    d = np.abs(got - want)[~odd]
+    d = np.abs(got[~odd] - want[~odd])
     t = np.broadcast_to(tol, want.shape)[~odd]
     assert (d <= t).all(), f"{what}: off by {d.max():.3e}, {float((d / np.maximum(t, 1e-300)).max()):.2f} of what is allowed"
 
@@ -261,7 +263,7 @@ def adjusted(x, history, n, rep, pre, fre, bias=None, hidden=None):
     return y
 
 
-LOGITS = [(1, 65, 128), (1, 1, 3), (3, 7, 1), (2, 1000, 50), (8, 50304, 1024), (5, 4097, 300), (2, 1024, 0), (64, 32768, 70), (300, 2052, 9), (17, 33333, 5000)]
+LOGITS = [(1, 65, 128), (1, 1, 3), (3, 7, 1), (2, 1000, 50), (8, 50304, 1024), (5, 4097, 300), (2, 1024, 0), (64, 32768, 70), (300, 2052, 9), (17, 33333, 5000), (1, 700, 70000)]
 
 
 @pytest.mark.gpu
@@ -501,6 +503,52 @@ def test_cache_attention(B, H, G, d, n, T, cap):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("tiles,waves,splits,stream", [(2, 4, 1, False), (2, 4, 3, False), (1, 8, 1, True), (1, 8, 2, False), (1, 4, 64, True), (2, 8, 1, False)])
+@pytest.mark.parametrize("B,H,G,d,n,T,cap", [(2, 2, 1, 64, 70, 150, 256), (1, 2, 3, 32, 300, 21, 512), (2, 1, 1, 64, 200, 1, 256), (1, 1, 2, 128, 700, 1, 768), (1, 2, 1, 40, 0, 33, 64)])
+def test_cache_attention_in_every_form(B, H, G, d, n, T, cap, tiles, waves, splits, stream, monkeypatch):
+    """The forms that the sizes choose between, forced on sizes where the others would run."""
+    if d > 64 and (tiles > 1 or waves > 4):
+        tiles, waves = 1, 4
+    monkeypatch.setattr(HIPLM, "attend_tiles", staticmethod(lambda *a: tiles))
+    monkeypatch.setattr(HIPLM, "attend_waves", staticmethod(lambda *a: waves))
+    monkeypatch.setattr(HIPLM, "attend_splits", staticmethod(lambda *a: splits))
+    monkeypatch.setattr(HIPLM, "attend_streams", staticmethod(lambda *a: stream))
+    if n % 64 and T > 64:
+        n = n // 64 * 64
+    test_cache_attention(B, H, G, d, n, T, cap)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("threads", [512, 1024])
+def test_cache_write_in_every_form(threads, monkeypatch):
+    monkeypatch.setattr(HIPLM, "write_threads", staticmethod(lambda *a: threads))
+    test_cache_holds_the_same_however_the_tokens_arrive(2, 64)
+    test_cache_holds_the_same_however_the_tokens_arrive(1, 130)
+    test_cache_rounds_exactly()
+
+
+@pytest.mark.gpu
+def test_cache_attention_of_many_rows():
+    """Enough query rows for two tiles a wavefront: the bits that a launch of its own, one tile a wavefront, gives for each sequence."""
+    require_gpu()
+    rng = np.random.default_rng(31)
+    B, H, d, T = 8, 12, 32, 256
+    assert HIPLM.attend_tiles(T, B * H, 32, 256) == 2 and HIPLM.attend_tiles(T, H, 32, 256) == 1
+    k, v = rows_of(rng, B, T, H * d)
+    q = rng.standard_normal((B, T, H * d)).astype(f32)
+    cache = nn.QuantizedKVCache(B, T, H, d)
+    cache.write(hip_tensor(k), hip_tensor(v))
+    y = cache.attend(hip_tensor(q)).numpy()
+    for b in range(0, B, 3):
+        one = nn.QuantizedKVCache(1, T, H, d)
+        one.write(hip_tensor(k[b:b + 1]), hip_tensor(v[b:b + 1]))
+        same(y[b:b + 1], one.attend(hip_tensor(q[b:b + 1])).numpy(), f"sequence {b}")
+    kk, vv = (held(a[0].reshape(T, H, d), T) for a in (k, v))
+    want, tol = attended(q[0].reshape(T, H, d), kk, vv, 0, d ** -0.5, H)
+    within(y[0].reshape(T, H, d), want, tol)
+
+
+@pytest.mark.gpu
 def test_cache_attention_of_extreme_queries():
     """Scores far apart (one token takes all the weight), tiny and huge queries, zeros."""
     require_gpu()
@@ -730,11 +778,11 @@ def test_cache_is_refused_off_the_device():
 
 
 def test_splits_and_slices():
-    """A part of the tokens has four blocks at least, and parts are made until the device is full, not further."""
-    assert HIPLM.attend_splits(4, 2, 256) == 1
-    assert HIPLM.attend_splits(1, 1000, 256) == 250
-    assert HIPLM.attend_splits(128, 512, 256) == 8
-    assert HIPLM.attend_splits(5000, 512, 256) == 1
+    """Parts are made from 8 blocks a wavefront on, their number grows with the root of the blocks, and they fill the device, not more."""
+    assert HIPLM.attend_splits(4, 2, 4, 256) == 1 and HIPLM.attend_splits(4, 31, 4, 256) == 1 and HIPLM.attend_splits(4, 63, 8, 256) == 1
+    assert HIPLM.attend_splits(1, 2048, 4, 256) == 32 and HIPLM.attend_splits(1, 1 << 18, 4, 256) == 64
+    assert HIPLM.attend_splits(128, 512, 4, 256) == 4 and HIPLM.attend_splits(192, 64, 8, 256) == 1
+    assert HIPLM.attend_splits(5000, 512, 4, 256) == 1
     assert HIPLM.adjust_items(1, 65, 256) == 4 and HIPLM.adjust_items(256, 128256, 256) == 32
     for B, V in ((1, 50304), (8, 50304), (64, 32000)):
         items = HIPLM.adjust_items(B, V, 256)

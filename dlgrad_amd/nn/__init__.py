@@ -127,18 +127,22 @@ def stack_parameters(tensors: list) -> None:
         t.data = part
 
 
-def self_attention_qkv(x: Tensor, wq: Tensor, wk: Tensor, wv: Tensor, n_head: int, scale: float, norm=None) -> Tensor:
+def self_attention_qkv(x: Tensor, wq: Tensor, wk: Tensor, wv: Tensor, n_head: int, scale: float, norm=None, rotary: "Rotary | None" = None) -> Tensor:
     """causal_self_attention(x @ wq^T, x @ wk^T, x @ wv^T, n_head, scale) for x (B, T, C) and three
     (C, C) weights: the projections and attention of examples/gpt.py:45-57.  When the weights are
     stacked in memory (stack_parameters) the hip device runs one projection and reads q, k, v out
     of its result in place (ops.SelfAttentionQKV).  norm: an RMSNorm to apply to x first; where the
-    one-projection form runs and the rows are short enough, that projection applies it."""
+    one-projection form runs and the rows are short enough, that projection applies it.  rotary: turns the
+    queries and keys by positions 0 .. T - 1, in place in the one-projection form."""
     if ops.use_fused_qkv_attention(x, wq, wk, wv, n_head):
         if norm is not None and ops.tile_norm_applies(x, wq, norm):
-            return ops.SelfAttentionQKV.execute(x, wq, wk, wv, norm.weight, n_head=n_head, scale=scale, eps=norm.eps)
-        return ops.SelfAttentionQKV.execute(x if norm is None else norm(x), wq, wk, wv, n_head=n_head, scale=scale)
+            return ops.SelfAttentionQKV.execute(x, wq, wk, wv, norm.weight, n_head=n_head, scale=scale, eps=norm.eps, rope=rotary)
+        return ops.SelfAttentionQKV.execute(x if norm is None else norm(x), wq, wk, wv, n_head=n_head, scale=scale, rope=rotary)
     if norm is not None:
         x = norm(x)
+    if rotary is not None:
+        q, k = rotary.pair(x.linear(wq, None), x.linear(wk, None), n_head)
+        return causal_self_attention(q, k, x.linear(wv, None), n_head, scale)
     return causal_self_attention(x.linear(wq, None), x.linear(wk, None), x.linear(wv, None), n_head, scale)
 
 

@@ -79,9 +79,14 @@ class Rotary:
             raise ValueError(f"rotary: no layout {layout!r} ('half' or 'interleaved')")
         if not 0 < rotated <= head_dim:
             raise ValueError(f"rotary: {rotated} of {head_dim} elements cannot turn")
-        self.head_dim, self.rotated, self.half, self.device = head_dim, rotated, layout == "half", as_device(device)
+        device = as_device(device)
+        if device is None:
+            raise ValueError("rotary: no such device")
+        self.head_dim, self.rotated, self.half = head_dim, rotated, layout == "half"
         self.frequencies, self.gain = rotary_frequencies(rotated, base, scaling, factor, trained)
         self._words, self._plans = None, {}
+        if device is Device.HIP:
+            self._table()
 
     def _table(self) -> Buffer:
         """The frequencies in turns per position as fractions of 2^64, on the device."""
@@ -89,7 +94,7 @@ class Rotary:
             from dlgrad_amd.runtime.hip import capturing
             from dlgrad_amd.runtime.hip_lm import HIPLM
             if capturing():
-                raise RuntimeError("rotary: use the object once outside a capture first (its table is uploaded then)")
+                raise RuntimeError("rotary: made for another device, its table cannot be uploaded inside a capture")
             turns = [int(round(float(f) / (2 * math.pi) % 1.0 * 2.0 ** 64)) % 2 ** 64 for f in self.frequencies]
             self._words = HIPLM.words(np.array(turns, dtype=np.uint64))
         return self._words

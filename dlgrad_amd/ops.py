@@ -650,21 +650,26 @@ class SelfAttentionQKV(OP):
     accumulator instead of three partial sums, so it differs from them by rounding."""
 
     def forward(self, x: Buffer, wq: Buffer, wk: Buffer, wv: Buffer, gain: Buffer | None = None, n_head: int = 1,
-                scale: float = 1.0, eps: float = 1e-6) -> Buffer:
-        """gain: the gain row of an RMSNorm that sits in front of the projection and is applied inside it."""
+                scale: float = 1.0, eps: float = 1e-6, rope=None) -> Buffer:
+        """gain: the gain row of an RMSNorm that sits in front of the projection and is applied inside it.
+        rope: an nn.Rotary that turns the queries and keys, where they lie in the projection, by positions 0 .. T - 1."""
         C = wq.shape[0]
-        self.x, self.n_head, self.scale, self.gain = x, n_head, scale, gain
+        self.x, self.n_head, self.scale, self.gain, self.rope = x, n_head, scale, gain, rope
         self.w = Buffer(wq.ptr, (3 * C, C), x.device)                    # the three matrices as one
         if gain is None:
             self.qkv, self.left = x.matmul_nt(self.w), x
         else:
             self.qkv, self.left, self.r = x.matmul_nt(self.w, norm=(gain, eps, True))
+        if rope is not None:
+            rope.turn_qkv_(self.qkv, n_head)
         self.y, self.p = self.qkv.causal_attention_qkv(n_head, scale)
         return self.y
 
     def _grads(self, upstream_grad: Buffer, plus: Buffer | None) -> tuple:
         C = self.w.shape[1]
         g = self.qkv.causal_attention_qkv_bwd(self.p, upstream_grad, self.n_head, self.scale, self.y)     # (B, T, 3C)
+        if self.rope is not None:
+            self.rope.turn_qkv_(g, self.n_head, back=True)
         dx, dw = product_pair(("nn", g, self.w), ("tn", g, self.left))
         dw = unbroadcast(dw, self.w.shape)                                                        # (3C, C)
         if dw.__class__ is PartialSum:

@@ -30,7 +30,13 @@ def _inference(fn):
 
 class GPTConfig:
     def __init__(self, vocab_size: int = 65, block_size: int = 128, n_layer: int = 6, n_head: int = 4,
-                 n_embd: int = 128, batch_size: int = 16, learning_rate: float = 1e-4, device: str = "hip") -> None:
+                 n_embd: int = 128, batch_size: int = 16, learning_rate: float = 1e-4, device: str = "hip",
+                 positions: str = "learned", cache: str = "float32") -> None:
+        """positions: "learned" (the reference's table) or "rotary" (nn.Rotary on queries and keys, no table); cache: "float32"
+        or "int8" (nn.QuantizedKVCache, hip only), for incremental decoding."""
+        if positions not in ("learned", "rotary") or cache not in ("float32", "int8"):
+            raise ValueError(f"GPTConfig: positions {positions!r}, cache {cache!r}")
+        self.positions, self.cache = positions, cache
         self.vocab_size, self.block_size, self.n_layer = vocab_size, block_size, n_layer
         self.n_head, self.n_embd, self.batch_size = n_head, n_embd, batch_size
         self.learning_rate, self.device = learning_rate, device
@@ -47,6 +53,7 @@ class CausalSelfAttention:
         self.c_proj = nn.Linear(c.n_embd, c.n_embd, bias=False, device=c.device)
         # same three parameters, placed back to back so that one product can serve all three projections
         nn.stack_parameters([self.q_proj.weight, self.k_proj.weight, self.v_proj.weight])
+        self.rope = nn.Rotary(self.head_dim, device=c.device) if c.positions == "rotary" else None
 
     def __call__(self, x: Tensor, cache: "KVCache | None" = None, layer: int = 0,
                  residual: Tensor | None = None, norm=None) -> Tensor:
@@ -59,11 +66,15 @@ class CausalSelfAttention:
             # q, k, v projections, split into heads, ((q @ k^T) * scale).masked_fill(mask, -inf).softmax(dim=3) @ v,
             # merge the heads (examples/gpt.py:45-57): one node on the hip device
             return self.c_proj(nn.self_attention_qkv(x, self.q_proj.weight, self.k_proj.weight, self.v_proj.weight,
-                                                     self.n_head, self.scale, norm), residual)
+                                                     self.n_head, self.scale, norm, self.rope), residual)
         q_lin, k_lin, v_lin = nn.project_qkv_row(x, self.q_proj.weight, self.k_proj.weight, self.v_proj.weight, norm)   # (B, T, C)
+        if self.rope is not None:
+            q_lin, k_lin = self.rope.pair(q_lin, k_lin, self.n_head, start=cache.start())
         if cache.length > 0:
             assert T == 1, "incremental attention takes one new position"
             cache.write(layer, k_lin, v_lin, cache.length)
+            if cache.quantized:
+                return self.c_proj(cache.store.attend(q_lin, self.scale, layer), residual)
             # the heads of q against the heads of everything cached (examples/gpt.py:58-63)
             y = nn.cached_attention(q_lin, cache.k[layer], cache.v[layer], cache.length + 1, self.n_head, self.scale)
         else:
@@ -84,7 +95,16 @@ class KVCache:
         shape = (c.block_size, batch, c.n_embd)
         self.k = [Tensor.full(shape, 0.0, device=c.device) for _ in range(c.n_layer)]
         self.v = [Tensor.full(shape, 0.0, device=c.device) for _ in range(c.n_layer)]
-        self.batch, self.length = batch, 0
+        self.batch, self.length, self.device = batch, 0, c.device
+
+    quantized = False
+
+    def start(self) -> Tensor | None:
+        """The position of the next token on the device, or None for 0."""
+        return Tensor.full((1, 1), float(self.length), device=self.device) if self.length else None
+
+    def advance(self, n: int) -> None:
+        self.length += n
 
     def write(self, layer: int, k: Tensor, v: Tensor, at: int) -> None:
         """k, v: (B, T, C) projections of positions at .. at+T-1."""
@@ -92,6 +112,28 @@ class KVCache:
         for store, new in ((self.k[layer], k), (self.v[layer], v)):
             rows = new if (B == 1 or T == 1) else new.transpose(0, 1)          # (T, B, C) order
             store[at:at + T].data.copy_(rows.data)
+
+
+class KVCache8:
+    """The same for GPTConfig(cache="int8"): nn.QuantizedKVCache, a quarter of the memory.  lengths: a (batch, 1) device tensor
+    with the number of tokens held, if the caller keeps one."""
+
+    quantized = True
+
+    def __init__(self, c: GPTConfig, batch: int, lengths: Tensor | None = None) -> None:
+        self.store = nn.QuantizedKVCache(batch, c.block_size, c.n_head, c.n_embd // c.n_head, c.n_layer, c.device, lengths)
+        self.batch, self.length = batch, 0
+
+    def start(self) -> Tensor | None:
+        return self.store.lengths if self.length else None
+
+    def advance(self, n: int) -> None:
+        self.length += n
+        self.store.advance(n)
+
+    def write(self, layer: int, k: Tensor, v: Tensor, at: int) -> None:
+        assert at == self.length
+        self.store.write(k, v, layer)
 
 
 class MLP:
@@ -132,7 +174,7 @@ class GPT:
     def __init__(self, c: GPTConfig) -> None:
         self.config = c
         self.wte = nn.Embedding(c.vocab_size, c.n_embd, device=c.device)
-        self.wpe = nn.Embedding(c.block_size, c.n_embd, device=c.device)
+        self.wpe = nn.Embedding(c.block_size, c.n_embd, device=c.device) if c.positions == "learned" else None
         self.blocks = [Block(c) for _ in range(c.n_layer)]
         self.ln_f = nn.RMSNorm(c.n_embd, device=c.device)
         self.lm_head = nn.Linear(c.n_embd, c.vocab_size, bias=False, device=c.device)
@@ -140,7 +182,7 @@ class GPT:
     def __call__(self, idx: Tensor, targets: Tensor | None = None):
         """idx, targets: (B, T) token ids stored as fp32.  Returns (logits, loss)."""
         B, T = idx.shape
-        x = nn.embed_tokens(self.wte, self.wpe, idx, _positions(T, idx.device))
+        x = self.wte(idx) if self.wpe is None else nn.embed_tokens(self.wte, self.wpe, idx, _positions(T, idx.device))
         for block in self.blocks:
             x = block(x)
         logits = nn.norm_linear(x, self.ln_f, self.lm_head.weight)
@@ -151,8 +193,11 @@ class GPT:
         return logits, loss
 
     # ---- incremental decoding with a device-resident key/value cache -----------------------------
-    def _hidden(self, idx: Tensor, pos: Tensor, cache: KVCache) -> Tensor:
-        x = self.wte(idx) + self.wpe(pos)
+    def new_cache(self, batch: int) -> "KVCache | KVCache8":
+        return (KVCache8 if self.config.cache == "int8" else KVCache)(self.config, batch)
+
+    def _hidden(self, idx: Tensor, pos: Tensor, cache: "KVCache | KVCache8") -> Tensor:
+        x = self.wte(idx) if self.wpe is None else self.wte(idx) + self.wpe(pos)      # (rotary positions come from the cache's length)
         for i, block in enumerate(self.blocks):
             x = block(x, cache, i)
         return self.ln_f(x)
@@ -163,9 +208,9 @@ class GPT:
         the last position as (B, 1, V) and the cache (the inference branch of
         examples/gpt.py:103-112, which slices the last position out on the host)."""
         B, T = idx.shape
-        cache = KVCache(self.config, B)
+        cache = self.new_cache(B)
         x = self._hidden(idx, _positions(T, idx.device), cache)
-        cache.length = T
+        cache.advance(T)
         C = x.shape[2]
         last = x.reshape((T, C))[T - 1:T] if B == 1 else x.transpose(0, 1)[T - 1:T]
         return self.lm_head(last.reshape((B, 1, C))), cache
@@ -176,25 +221,27 @@ class GPT:
         the cache and returns logits (B, 1, V) (examples/gpt.py:114-136)."""
         assert new_idx.shape[1] == 1, "incremental forward expects a single token"
         x = self._hidden(new_idx, pos, cache)
-        cache.length += 1
+        cache.advance(1)
         return self.lm_head(x)
 
     def generate(self, first_token: int, max_new_tokens: int, temperature: float = 1.0, u=None,
-                 reference_positions: bool = STRICT_REFERENCE) -> list[int]:
+                 reference_positions: bool = STRICT_REFERENCE, penalties: dict | None = None) -> list[int]:
         """The reference's generate (examples/gpt.py:169-226) with its sampling: the key/value-cache loop of
         generate_greedy_cached, each token drawn on the host from softmax(logits / temperature) of the
         downloaded logits (np.random.choice there; helpers.sample_from_logits here, which is choice() with
         its uniform draw given).  u: max_new_tokens uniform numbers in [0, 1), one per token (a tensor or an
-        array); drawn from the device's seeded generator (dlgrad_amd.manual_seed) when None."""
+        array); drawn from the device's seeded generator (dlgrad_amd.manual_seed) when None.
+        penalties: see generate_greedy_cached."""
         if u is None:
             u = Tensor.uniform((max(max_new_tokens, 1),), device=self.config.device)
         u = np.asarray(u.numpy() if isinstance(u, Tensor) else u, dtype=np.float32).reshape(-1)
         if u.size < max_new_tokens or not temperature > 0:
             raise ValueError("generate: one uniform number per new token and a positive temperature are needed")
-        return self.generate_greedy_cached(first_token, max_new_tokens, reference_positions, (float(temperature), u))
+        return self.generate_greedy_cached(first_token, max_new_tokens, reference_positions, (float(temperature), u), penalties)
 
     def generate_greedy_cached(self, first_token: int, max_new_tokens: int,
-                               reference_positions: bool = STRICT_REFERENCE, sampling: tuple | None = None) -> list[int]:
+                               reference_positions: bool = STRICT_REFERENCE, sampling: tuple | None = None,
+                               penalties: dict | None = None) -> list[int]:
         """The control flow of the reference's generate (examples/gpt.py:169-226) with argmax in
         place of sampling (sampling = (temperature, uniform numbers): drawn on the host instead, see
         generate): a full forward when there is no cache, one-token steps after it,
@@ -202,7 +249,9 @@ class GPT:
         dropped and every further token is a full forward over the last block_size tokens.
         reference_positions reproduces its position id for an incremental token, the sequence
         length *including* that token (one more than the token's index, examples/gpt.py:199).
-        Tokens, cache and argmax stay on the device; the ids come back in one download."""
+        Tokens, cache and argmax stay on the device; the ids come back in one download.
+        penalties: keyword arguments of nn.adjust_logits (repetition, presence, frequency, bias, hidden), applied to the
+        logits of every token with the tokens so far as its history."""
         c = self.config
         seq = Tensor.full((max_new_tokens + 1, 1), float(int(first_token)), device=c.device)
         n, start, cache = 1, 0, None                       # tokens so far; first token of the context window
@@ -215,6 +264,9 @@ class GPT:
                 length = n - start
                 pos = Tensor.full((1, 1), float(length if reference_positions else length - 1), device=c.device)
                 logits = self.forward_incremental(seq[n - 1:n], pos, cache)
+            if penalties is not None:
+                with nn.inference():
+                    logits = nn.adjust_logits(logits.reshape((1, c.vocab_size)), seq[0:n].reshape((1, n)), **penalties)
             if sampling is None:
                 nxt = logits.reshape((1, c.vocab_size)).argmax(1)                       # (1, 1), on the device
             else:
@@ -264,8 +316,10 @@ class StaticDecoder:
     softmax sums) and, with reference_positions=False, as full recompute (generate_greedy)."""
 
     def __init__(self, model: GPT, reference_positions: bool = STRICT_REFERENCE, capacity: int | None = None,
-                 temperature: float | None = None) -> None:
-        """temperature: None decodes greedily; a positive number draws every token from
+                 temperature: float | None = None, penalties: dict | None = None) -> None:
+        """penalties: keyword arguments of nn.adjust_logits (repetition, presence, frequency, bias, hidden; tensors stay where they
+        are, so a captured step sees what is written into them), applied to the logits of every token with the tokens so far.
+        temperature: None decodes greedily; a positive number draws every token from
         softmax(logits / temperature) as the reference's generate does (examples/gpt.py:209-221, :258-266),
         with the uniform numbers of the device's seeded generator (dlgrad_amd.manual_seed), one per token,
         made before the first step (reset) and kept on the device: on the hip device the draw is the last
@@ -276,9 +330,10 @@ class StaticDecoder:
         self.temperature = None if temperature is None else float(temperature)
         self.model, self.reference_positions = model, reference_positions
         self.capacity = int(capacity) if capacity is not None else 2 * c.block_size + 1     # tokens the buffer holds
-        self.cache = KVCache(c, 1)
+        self.penalties = penalties
         self.tok = Tensor.full((1, 1), 0.0, device=c.device)          # token to feed
         self.slot = Tensor.full((1, 1), 0.0, device=c.device)         # its index = cache row to write
+        self.cache = KVCache8(c, 1, self.slot) if c.cache == "int8" else KVCache(c, 1)
         self.seq = Tensor.full((max(self.capacity, c.block_size + 1), 1), 0.0, device=c.device)
         self.u = Tensor.full((self.seq.shape[0],), 0.0, device=c.device) if self.temperature is not None else None
         self.graph = None
@@ -301,8 +356,17 @@ class StaticDecoder:
         first[0, 0] = first_token
         self.seq.data.upload_(first)
 
-    def _attend(self, attn: CausalSelfAttention, x: Tensor, norm, layer: int, hidden: Tensor, residual: Tensor) -> Tensor:
+    def _attend(self, attn: CausalSelfAttention, x: Tensor, norm, layer: int, hidden: Tensor | None, residual: Tensor) -> Tensor:
         T = self.model.config.block_size
+        if attn.rope is not None or self.cache.quantized:
+            q, k, v = nn.project_qkv_row(x, attn.q_proj.weight, attn.k_proj.weight, attn.v_proj.weight, norm)
+            if attn.rope is not None:
+                q, k = attn.rope.pair(q, k, attn.n_head, start=self.slot)
+            if self.cache.quantized:
+                self.cache.store.write(k, v, layer)
+                return attn.c_proj(self.cache.store.attend(q, attn.scale, layer), residual)
+            self.cache.k[layer].data.row_store_(k.data, self.slot.data, also=(self.cache.v[layer].data, v.data))
+            return attn.c_proj(nn.cached_attention(q, self.cache.k[layer], self.cache.v[layer], T, attn.n_head, attn.scale, hidden), residual)
         q = nn.decode_query_row(x, attn.q_proj.weight, attn.k_proj.weight, attn.v_proj.weight, norm,
                                 self.cache.k[layer], self.cache.v[layer], self.slot)     # (k and v go straight to their cache rows)
         if q is None:
@@ -314,6 +378,8 @@ class StaticDecoder:
     def _append(self, logits: Tensor) -> None:
         """logits (1, V) of the newest position: its argmax -- or, for a sampling decoder, the token that u[slot] draws
         from softmax(logits / temperature) -- becomes seq[slot + 1] and the next token; slot advances."""
+        if self.penalties is not None:
+            logits = nn.adjust_logits(logits, self.seq.reshape((1, self.seq.shape[0])), self.slot + 1.0, **self.penalties)
         if self.temperature is not None:
             if nn.decode_sample(logits, self.u, self.tok, self.slot, self.seq, self.temperature):     # one launch
                 return
@@ -336,9 +402,12 @@ class StaticDecoder:
         token, and advances slot.  Reads and writes device memory only."""
         m, c = self.model, self.model.config
         slot = self.slot
-        got = nn.decode_input(m.wte.weight, m.wpe.weight, self.tok, slot, c.block_size, self.reference_positions)
+        got = None if m.wpe is None else nn.decode_input(m.wte.weight, m.wpe.weight, self.tok, slot, c.block_size, self.reference_positions)
         if got is not None:
             x, hidden = got
+        elif m.wpe is None:                                 # rotary: positions are the tokens' indices, whatever reference_positions says
+            x = m.wte(self.tok)
+            hidden = None if self.cache.quantized else Tensor.arange((1, c.block_size), device=c.device) > slot
         else:
             # the reference numbers an incremental token one too high (examples/gpt.py:199); token 0 is a full forward there
             pos = slot + slot.clamp(min=0, max=1) if self.reference_positions else slot
@@ -355,7 +424,7 @@ class StaticDecoder:
         at positions 0 .. block_size - 1; the argmax of the last position becomes token slot + 1."""
         m, c = self.model, self.model.config
         T = c.block_size
-        x = nn.decode_window_input(m.wte.weight, m.wpe.weight, self.seq, self.slot, T)     # window gathered and embedded in one launch
+        x = None if m.wpe is None else nn.decode_window_input(m.wte.weight, m.wpe.weight, self.seq, self.slot, T)     # window gathered and embedded in one launch
         if x is None:
             where = Tensor.arange((1, T), device=c.device) + (self.slot - float(T - 1))    # indices into the token buffer
             window = Tensor.embedding(self.seq, where).reshape((1, T))                      # the tokens themselves

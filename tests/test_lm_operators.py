@@ -787,3 +787,141 @@ def test_splits_and_slices():
     for B, V in ((1, 50304), (8, 50304), (64, 32000)):
         items = HIPLM.adjust_items(B, V, 256)
         assert items == 4 or B * -(-V // (256 * items)) >= 512
+
+
+# ================================================================ in the GPT of the examples
+TINY = dict(vocab_size=33, block_size=96, n_layer=2, n_head=2, n_embd=64, batch_size=3)
+
+
+def gpt(device, seed=3, std=0.2, **kw):
+    from examples import gpt as G
+    model = G.GPT(G.GPTConfig(device=device, **{**TINY, **kw}))
+    G.init_weights_(model, seed, std)
+    return model
+
+
+def test_gpt_options_and_parameters():
+    from examples import gpt as G
+    for bad in (dict(positions="other"), dict(cache="int4")):
+        with pytest.raises(ValueError):
+            G.GPTConfig(**bad)
+    learned, rotary = gpt("cpu"), gpt("cpu", positions="rotary")
+    names = set(nn.utils.get_state_dict(learned))
+    assert names - set(nn.utils.get_state_dict(rotary)) == {"wpe.weight"}
+    assert len(nn.utils.get_parameters(rotary)) == len(names) - 1
+
+
+def test_rotary_gpt_decodes_as_it_recomputes_on_the_cpu():
+    """The cached, the fixed-shape and the recomputing decoders agree, with penalties too, inside the window and beyond it."""
+    from examples import gpt as G
+    model = gpt("cpu", positions="rotary", block_size=16)
+    want = model.generate_greedy(3, 12)
+    assert model.generate_greedy_cached(3, 12) == want
+    assert G.StaticDecoder(model).generate(3, 22)[:13] == want
+    kw = dict(repetition=1.7, presence=0.3, frequency=0.2)
+    got = G.StaticDecoder(model, penalties=kw).generate(3, 22)
+    assert got[:13] == model.generate_greedy_cached(3, 12, penalties=kw) != want
+    hidden = np.ones(33, f32)
+    hidden[[5, 6]] = 0
+    assert set(model.generate(3, 12, u=np.linspace(0, 0.99, 12), penalties=dict(hidden=Tensor(hidden)))[1:]) <= {5, 6}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [64, 96])
+def test_rotary_gpt_trains_as_on_the_cpu(T):
+    """Loss and every gradient of a step against the CPU composition: 1e-4, what this package asks of a whole step in fp32."""
+    require_gpu()
+    rng = np.random.default_rng(T)
+    ids, targets = (rng.integers(0, 33, (3, T)).astype(f32) for _ in range(2))
+    got = {}
+    for device in ("cpu", "hip"):
+        model = gpt(device, positions="rotary", std=0.05)
+        _, loss = model(Tensor(ids, device=device), Tensor(targets, device=device))
+        loss.backward()
+        got[device] = (float(loss.numpy()), {k: p.grad.numpy() for k, p in nn.utils.get_state_dict(model).items()})
+    if hip.COMPILE_ONLY:
+        return
+    assert abs(got["hip"][0] - got["cpu"][0]) <= 1e-4 * abs(got["cpu"][0])
+    for name, want in got["cpu"][1].items():
+        assert np.abs(got["hip"][1][name] - want).max() <= 1e-4 * np.abs(want).max(), name
+
+
+@pytest.mark.gpu
+def test_rotary_inside_the_projection_is_rotary_after_it(monkeypatch):
+    """Turned in place in the stacked projection: the context has the bits of three projections turned as tensors; and the
+    gradient of x is that of the same composition to the rounding of one accumulator against three."""
+    require_gpu()
+    rng = np.random.default_rng(2)
+    B, T, h, d = 2, 40, 4, 16
+    C = h * d
+    rope = nn.Rotary(d, layout="interleaved")
+    x = rng.standard_normal((B, T, C)).astype(f32)
+    w = [(rng.standard_normal((C, C)) * C ** -0.5).astype(f32) for _ in range(3)]
+    g = rng.standard_normal((B, T, C)).astype(f32)
+    out = []
+    for stacked in (True, False):
+        xt, ws = hip_tensor(x, True), [hip_tensor(a, True) for a in w]
+        if stacked:
+            nn.stack_parameters(ws)
+            assert ops.use_fused_qkv_attention(xt, *ws, h)
+        else:
+            monkeypatch.setattr(ops, "use_fused_qkv_attention", lambda *a: False)
+        y = nn.self_attention_qkv(xt, *ws, h, d ** -0.5, rotary=rope)
+        (y * hip_tensor(g)).sum().backward()
+        out.append([y.numpy(), xt.grad.numpy(), *[a.grad.numpy() for a in ws]])
+    if hip.COMPILE_ONLY:
+        return
+    same(out[0][0], out[1][0], "context")
+    for a, b in zip(out[0][1:], out[1][1:]):
+        assert np.abs(a - b).max() <= 3 * C * EPS * np.abs(b).max()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("positions", ["learned", "rotary"])
+@pytest.mark.parametrize("cache", ["float32", "int8"])
+def test_gpt_decodes_with_every_combination(positions, cache):
+    """Rotary positions, the 8-bit cache and penalties together, as a decoder uses them: eager steps, a captured graph and -- while no block of
+    the cache is full, so that it holds what the fp32 cache holds -- the CPU's decoder give the same tokens."""
+    require_gpu()
+    from examples import gpt as G
+    penalties = dict(repetition=1.3, presence=0.2, frequency=0.1)
+    model = gpt("hip", positions=positions, cache=cache)
+    eager = model.generate_greedy_cached(7, 90, False, penalties=penalties)
+    for temperature in (None, 0.8):
+        u = np.random.default_rng(1).random(120).astype(f32)
+        dec = G.StaticDecoder(model, reference_positions=False, capacity=121, temperature=temperature, penalties=penalties)
+        plain = dec.generate(7, 110, u) if temperature else dec.generate(7, 110)
+        dec.capture()
+        for _ in range(2):
+            tokens = dec.generate(7, 110, u) if temperature else dec.generate(7, 110)
+            if not hip.COMPILE_ONLY:
+                assert tokens == plain
+        dec.close()
+        if not temperature and not hip.COMPILE_ONLY:
+            assert tokens[:91] == eager
+    if not hip.COMPILE_ONLY:
+        cpu = gpt("cpu", positions=positions).generate_greedy_cached(7, 60, False, penalties=penalties)
+        assert tokens is not None and eager[:61] == cpu
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("first", [20, 64, 70])
+def test_gpt_prompt_into_the_quantized_cache(first):
+    """A batch of prompts, then single tokens, against an fp32 cache that holds the values the 8-bit one stands for: 1e-4, what this
+    package asks of a whole pass in fp32."""
+    require_gpu()
+    from examples import gpt as G
+    rng = np.random.default_rng(4)
+    ids = rng.integers(0, 33, (3, 90)).astype(f32)
+    model, plain = gpt("hip", cache="int8", positions="rotary"), gpt("hip", positions="rotary")
+    got, cache = model.prefill(hip_tensor(ids[:, :first]))
+    want, _ = plain.prefill(hip_tensor(ids[:, :first]))
+    same(got.numpy(), want.numpy(), "the prompt itself attends in fp32")
+    wide = G.KVCache(plain.config, 3)
+    for layer in range(2):
+        wide.write(layer, *cache.store.read(first, layer), 0)
+    wide.advance(first)
+    for t in range(first, first + 20 if first < 64 else 90):
+        got, want = (m.forward_incremental(hip_tensor(ids[:, t:t + 1]), hip_tensor([[t]]), c).numpy() for m, c in ((model, cache), (plain, wide)))
+        if not hip.COMPILE_ONLY:
+            assert np.abs(got - want).max() <= 1e-4 * np.abs(want).max(), t

@@ -3949,3 +3949,12 @@ extern "C" __global__ __launch_bounds__(256) void {name}(const float* __restrict
 {body}}}
 """
     return src, name, _fmt("P", "P", "P", "P", "P", "P", "P", "I", "8f")
+
+
+def __getattr__(name: str):
+    """The generators of lm_kernel.py, which builds on this module, by their names: kernels are listed and compiled as this module's."""
+    if name.endswith("_kernel"):
+        from dlgrad_amd.codegen import lm_kernel
+        if name in vars(lm_kernel):
+            return vars(lm_kernel)[name]
+    raise AttributeError(f"module {__name__!r} has no attribute {name!r}")

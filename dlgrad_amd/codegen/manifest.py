@@ -43,16 +43,11 @@ def merge(entries, path: str = PATH) -> None:
         f.write("[\n" + ",\n".join(json.dumps(r) for r in rows) + "\n]\n")
 
 
-def generator(name: str):
-    """The kernel generator of that name, in whichever module of this package it lives."""
-    from dlgrad_amd.codegen import hip_kernel, lm_kernel
-    return getattr(lm_kernel if hasattr(lm_kernel, name) else hip_kernel, name)
-
-
 def _compile_one(job) -> str:
+    from dlgrad_amd.codegen import hip_kernel as K
     from dlgrad_amd.runtime import hip
     (gen, params), force = job
-    src, name, _ = generator(gen)(*params)
+    src, name, _ = getattr(K, gen)(*params)
     hip.code_object(src, name, force=force)
     return name
 

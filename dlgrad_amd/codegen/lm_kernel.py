@@ -37,7 +37,7 @@ static __device__ __forceinline__ u32 turn_of(int p, u64 f) {
 
 
 @cache
-def rotary_kernel(half: bool, vec: bool) -> tuple[str, str, str]:
+def rotary_kernel(half: bool, vec: bool, stream: bool = False) -> tuple[str, str, str]:
     """y = x with the first `rot` of the d elements of every head turned pair by pair: (a, b) becomes
     gain * (a cos w - b sin w, a sin w + b cos w) with w = position * frequency of the pair, the other elements
     copied.  half: pair i is elements i and i + rot / 2; otherwise 2 i and 2 i + 1.  back = 1 turns by -w, which
@@ -52,24 +52,27 @@ def rotary_kernel(half: bool, vec: bool) -> tuple[str, str, str]:
     writes it).  A thread takes one group of pairs (vec: 16-byte accesses; 4 pairs with half, 2 without) of up to
     four heads, H / 4 apart so that neighbouring lanes touch neighbouring heads: the loads are issued first and the
     angles, once for all four heads, are computed while they are in flight.  grid.z = 2 turns a second tensor
-    (keys beside queries) in the same launch.  Bound by memory: 8 bytes an element."""
-    name = f"rotary_{'half' if half else 'pairs'}_{'v4' if vec else 'v1'}"
+    (keys beside queries) in the same launch.  stream: loads and stores that bypass the caches, for tensors larger than they
+    are.  Bound by memory: 8 bytes an element (30001 rows of 32 + 8 heads of 128: 206 us, 6.0 TB/s; 218 us through the caches)."""
+    assert vec or not stream
+    name = f"rotary_{'half' if half else 'pairs'}_{'v4' if vec else 'v1'}{'_nt' if stream else ''}"
+    get = (lambda at: f"ld4_stream(reinterpret_cast<const float4*>({at}))") if stream else (lambda at: f"*reinterpret_cast<const float4*>({at})")      # noqa: E731
+    put = ((lambda at, v: f"{{ const v4f o4 = {{{v}}}; __builtin_nontemporal_store(o4, reinterpret_cast<v4f*>({at})); }}") if stream
+           else (lambda at, v: f"*reinterpret_cast<float4*>({at}) = make_float4({v});"))                                            # noqa: E731
     W = (4 if half else 2) if vec else 1                 # pairs of a rotating unit
     if half:
-        load = ("const float4 a = *reinterpret_cast<const float4*>(xr + off + j), b = *reinterpret_cast<const float4*>(xr + off + hr + j);"
+        load = (f"const float4 a = {get('xr + off + j')}, b = {get('xr + off + hr + j')};"
                 if vec else "const float a = xr[off + j], b = xr[off + hr + j];")
         keep = ("va[n][0] = a.x; va[n][1] = a.y; va[n][2] = a.z; va[n][3] = a.w; vb[n][0] = b.x; vb[n][1] = b.y; vb[n][2] = b.z; vb[n][3] = b.w;"
                 if vec else "va[n][0] = a; vb[n][0] = b;")
-        store = ("*reinterpret_cast<float4*>(yr + off + j) = make_float4(oa[0], oa[1], oa[2], oa[3]); "
-                 "*reinterpret_cast<float4*>(yr + off + hr + j) = make_float4(ob[0], ob[1], ob[2], ob[3]);"
-                 if vec else "yr[off + j] = oa[0]; yr[off + hr + j] = ob[0];")
+        store = (put("yr + off + j", "oa[0], oa[1], oa[2], oa[3]") + " " + put("yr + off + hr + j", "ob[0], ob[1], ob[2], ob[3]") if vec else "yr[off + j] = oa[0]; yr[off + hr + j] = ob[0];")
     else:
-        load = ("const float4 a = *reinterpret_cast<const float4*>(xr + off + 2u * j);" if vec
+        load = (f"const float4 a = {get('xr + off + 2u * j')};" if vec
                 else "const float a = xr[off + 2u * j], b = xr[off + 2u * j + 1u];")
         keep = ("va[n][0] = a.x; vb[n][0] = a.y; va[n][1] = a.z; vb[n][1] = a.w;" if vec else "va[n][0] = a; vb[n][0] = b;")
-        store = ("*reinterpret_cast<float4*>(yr + off + 2u * j) = make_float4(oa[0], ob[0], oa[1], ob[1]);" if vec
+        store = (put("yr + off + 2u * j", "oa[0], ob[0], oa[1], ob[1]") if vec
                  else "yr[off + 2u * j] = oa[0]; yr[off + 2u * j + 1u] = ob[0];")
-    copy = ("*reinterpret_cast<float4*>(yr + off + c) = *reinterpret_cast<const float4*>(xr + off + c);" if vec else "yr[off + c] = xr[off + c];")
+    copy = (f"const float4 a = {get('xr + off + c')}; " + put("yr + off + c", "a.x, a.y, a.z, a.w") if vec else "yr[off + c] = xr[off + c];")
     CW = 4 if vec else 1
     src = f"""{PRELUDE}{_ANGLES}
 extern "C" __global__ __launch_bounds__(256) void {name}(const float* x0, float* y0, const float* x1, float* y1,
@@ -152,7 +155,7 @@ def adjust_logits_kernel(items: int, vec: bool, packed: bool) -> tuple[str, str,
     no sort.  packed: two 16-bit counters to a word, for histories of at most 65535 -- half the LDS, twice the blocks on a
     compute unit.  The first 16 entries a thread walks and its logits are loaded before the counters are cleared, so all of
     these reads are on their way together.  vec: 16-byte accesses (V % 4 == 0)."""
-    assert items in (4, 8, 16, 32)
+    assert items in (4, 8, 16)
     name = f"adjust_logits_i{items}_{'v4' if vec else 'v1'}{'_h' if packed else ''}"
     W = 4 if vec else 1
     NV = items // W

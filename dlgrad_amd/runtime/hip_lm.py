@@ -12,7 +12,7 @@ from dlgrad_amd.codegen import lm_kernel as K
 from dlgrad_amd.device import Device
 from dlgrad_amd.dispatch import dispatcher
 from dlgrad_amd.helpers import CustomOps
-from dlgrad_amd.runtime.hip import DevicePtr, _addr, _PlanCache, _upload, alloc, field_offset, kernel, launch, launch_out, props
+from dlgrad_amd.runtime.hip import NT_STORE_MIN_ELEMENTS, DevicePtr, _addr, _PlanCache, _upload, alloc, field_offset, kernel, launch, launch_out, props
 
 STREAM_BYTES = 1 << 28       # the Infinity Cache
 EXACT_WHOLE = 1 << 24        # whole numbers up to here are exact in fp32
@@ -82,6 +82,7 @@ class HIPLM:
         if n_starts not in (0, 1, batch):
             raise ValueError(f"rotary: {n_starts} starts for {batch} sequences")
         two = len(sizes) - 1
+        numel0, numel1 = rows * sizes[0][1] * d, rows * sizes[two][1] * d
         out_pitch = [p if inplace else h * d for _, h, p in sizes]
         unit = 8 if half else 4                                        # elements of a unit of pairs in 16-byte accesses
         wide = rot % unit == 0 and d % 4 == 0 and all(p % 4 == 0 for _, _, p in sizes)
@@ -92,12 +93,13 @@ class HIPLM:
             if blocks >= 2 ** 31:
                 raise ValueError(f"rotary: {rows} rows exceed the grid")
             return (blocks, 1, 1 + two)
+        stream = not inplace and numel0 + two * numel1 >= NT_STORE_MIN_ELEMENTS
 
         def variant(vec: bool) -> list:
             v = [None, grid(vec), None]
 
             def load():
-                v[0] = kernel(K.rotary_kernel, half, vec)
+                v[0] = kernel(K.rotary_kernel, half, vec, stream and vec)
                 return v[0]
             v[2] = load
             return v
@@ -105,8 +107,6 @@ class HIPLM:
         first = variant(True) if wide else narrow
         tail = (rows, T, per, sizes[0][1], sizes[two][1], d, rot, sizes[0][2], sizes[two][2], out_pitch[0], out_pitch[two],
                 T if n_positions == batch * T else 0, 1 if n_starts == batch else 0, int(back), float(gain))
-        numel0, numel1 = rows * sizes[0][1] * d, rows * sizes[two][1] * d
-
         def run(x0: DevicePtr, x1: DevicePtr | None, table: int, pos: int, start: int) -> tuple:
             a0 = x0.addr
             a1 = x1.addr if two else a0
@@ -284,8 +284,9 @@ class HIPLM:
     @staticmethod
     def adjust_items(B: int, V: int, compute_units: int) -> int:
         """Logits per thread of the adjustment: every block walks its row's whole history, so long slices of the vocabulary save
-        walks -- as long as there are two blocks for every compute unit."""
-        for items in (32, 16, 8):
+        walks -- as long as there are two blocks for every compute unit (256 x 128256 logits, 4000 said: 59 us with 8, 52 with 16, 55
+        with 32; 32 x 128256, 300 said: 9.3, 9.7, 11.1)."""
+        for items in (16, 8):
             if B * -(-V // (256 * items)) >= 2 * compute_units:
                 return items
         return 4

@@ -157,6 +157,21 @@ def test_rotary_pair_and_four_dimensions():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+def test_rotary_beyond_the_caches_has_the_same_bits(layout, monkeypatch):
+    """The form for large tensors, which bypasses the caches, forced on a small one."""
+    require_gpu()
+    from dlgrad_amd.runtime import hip_lm
+    rng = np.random.default_rng(12)
+    q, k = rng.standard_normal((2, 33, 6 * 48)).astype(f32), rng.standard_normal((2, 33, 2 * 48)).astype(f32)
+    want = [t.numpy() for t in nn.Rotary(48, 32, layout=layout).pair(hip_tensor(q), hip_tensor(k), 6, 2)]
+    monkeypatch.setattr(hip_lm, "NT_STORE_MIN_ELEMENTS", 1)
+    monkeypatch.setattr(hip_lm, "_rotary_plans", {})
+    for a, b in zip(nn.Rotary(48, 32, layout=layout).pair(hip_tensor(q), hip_tensor(k), 6, 2), want):
+        same(a.numpy(), b)
+
+
+@pytest.mark.gpu
 def test_rotary_of_unaligned_views_and_of_nothing():
     require_gpu()
     rng = np.random.default_rng(2)
@@ -783,7 +798,7 @@ def test_splits_and_slices():
     assert HIPLM.attend_splits(1, 2048, 4, 256) == 32 and HIPLM.attend_splits(1, 1 << 18, 4, 256) == 64
     assert HIPLM.attend_splits(128, 512, 4, 256) == 4 and HIPLM.attend_splits(192, 64, 8, 256) == 1
     assert HIPLM.attend_splits(5000, 512, 4, 256) == 1
-    assert HIPLM.adjust_items(1, 65, 256) == 4 and HIPLM.adjust_items(256, 128256, 256) == 32
+    assert HIPLM.adjust_items(1, 65, 256) == 4 and HIPLM.adjust_items(256, 128256, 256) == 16
     for B, V in ((1, 50304), (8, 50304), (64, 32000)):
         items = HIPLM.adjust_items(B, V, 256)
         assert items == 4 or B * -(-V // (256 * items)) >= 512

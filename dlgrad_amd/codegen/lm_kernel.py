@@ -270,6 +270,23 @@ static __device__ __forceinline__ void cache8_extent(const float* __restrict__ l
 """
 
 
+def _cache8_layout(DP: int) -> str:
+    """Where a block of 64 tokens by DP columns keeps its bytes: in the order in which the wavefront of cache8_attend_kernel reads
+    them, so that each of its loads is one run of memory.  Lane r + 16 g (r < 16, g < 4) takes of the keys, for token tile u, the quarter
+    g .. of the columns of token 16 (r / 4) + 4 u + r % 4, 16 bytes at a time (8 where a quarter is no multiple of 16); of the
+    values, for columns 16 dt + r, the tokens 16 g .. 16 g + 15."""
+    Q4 = DP // 4
+    w = 16 if Q4 % 16 == 0 else 8
+    return f"""
+#define DP {DP}u
+static __device__ __forceinline__ u32 key_at(u32 row, u32 c) {{
+    const u32 g = c / {Q4}u, i = c % {Q4}u;
+    return ((row >> 2) & 3u) * {64 * Q4}u + (i / {w}u) * {64 * w}u + (g * 16u + ((row >> 4) << 2) + (row & 3u)) * {w}u + i % {w}u;
+}}
+static __device__ __forceinline__ u32 value_at(u32 row, u32 c) {{ return (c >> 4) * 1024u + ((row >> 4) * 16u + (c & 15u)) * 16u + (row & 15u); }}
+"""
+
+
 @cache
 def cache8_write_kernel(DP: int, vec: bool, NT: int = 1024) -> tuple[str, str, str]:
     """New key and value rows k, v (B, T, H * d) into the 8-bit cache of one layer, at positions lengths[b] .. of each sequence
@@ -277,8 +294,8 @@ def cache8_write_kernel(DP: int, vec: bool, NT: int = 1024) -> tuple[str, str, s
 
     A block of 64 tokens of one head is quantised when its last token arrives, and never again: scale = max |x| / 127
     in 32 bits, code = x / scale to the nearest whole number, ties to even.  Until then its rows stay fp32 in the tail, so what
-    the cache holds depends on the tokens alone and not on the calls that brought them.  Key codes lie as [64][DP] bytes, value
-    codes transposed, [DP][64], each code + 128; two tails of 64 rows per head, block i's in tail i & 1.
+    the cache holds depends on the tokens alone and not on the calls that brought them.  A code is a byte, code + 128, where
+    _cache8_layout says; there are two tails of 64 rows per head, block i's is tail i & 1.
 
     The quotient is rounded exactly: q = rint(x * (1 / scale)) may be off by one next to a half.  There x - q * scale, which is
     representable (both are multiples of the unit of the smaller one, and it is below two scales), comes without error from
@@ -309,9 +326,7 @@ def cache8_write_kernel(DP: int, vec: bool, NT: int = 1024) -> tuple[str, str, s
                 if (c0 + 2u < d) { fk.z = pk[c0 + 2u]; fv.z = pv[c0 + 2u]; }
                 if (c0 + 3u < d) { fk.w = pk[c0 + 3u]; fv.w = pv[c0 + 3u]; }
             }"""
-    src = f"""{PRELUDE}{_CACHE8}
-#define DP {DP}u
-#define C4 {DP // 4}u
+    src = f"""{PRELUDE}{_CACHE8}{_cache8_layout(DP)}#define C4 {DP // 4}u
 // four codes + 128 in the bytes of a word
 static __device__ __forceinline__ u32 codes_of(float4 f, float s, float inv, float up) {{
     const float x[4] = {{f.x * up, f.y * up, f.z * up, f.w * up}};
@@ -341,7 +356,7 @@ extern "C" __global__ __launch_bounds__({NT}) void {name}(const float* __restric
         const float* __restrict__ lengths, const float* __restrict__ counts,
         unsigned char* __restrict__ kc, unsigned char* __restrict__ vc, float* __restrict__ scales, float* tail_k, float* tail_v,
         u32 T, u32 H, u32 d, u32 NB, u32 kp, u32 vp) {{
-    __shared__ u32 vt[DP * 17u];                                        // value codes of the block, rows of 64 bytes, 68 apart
+    __shared__ __attribute__((aligned(16))) u32 kt[DP * 16u], vt[DP * 16u];       // the block's bytes
     __shared__ float sk[{NT // 64}], sv[{NT // 64}];
     __shared__ u32 bad[64];
     const u32 t = threadIdx.x, lane = t & 63u, h = blockIdx.y, b = blockIdx.z;
@@ -408,21 +423,24 @@ extern "C" __global__ __launch_bounds__({NT}) void {name}(const float* __restric
             // a scale below 2^-60 has no finite reciprocal or an inexact remainder: both sides times 2^64, exactly
             const float upk = ak < 8.6736174e-19f ? 18446744073709551616.0f : 1.0f, upv = av < 8.6736174e-19f ? 18446744073709551616.0f : 1.0f;
             const float s_k = ak * upk, s_v = av * upv, ik = ak > 0.0f ? 1.0f / s_k : 0.0f, iv = av > 0.0f ? 1.0f / s_v : 0.0f;
-            unsigned char* __restrict__ kb = kc + at * (64u * DP);
             unsigned char* vt8 = reinterpret_cast<unsigned char*>(vt);
             #pragma unroll
             for (u32 it = 0; it < {IT}u; ++it) {{
                 const u32 row = (it * {NT}u + t) / C4, c0 = (it * {NT}u + t) % C4 * 4u;
                 if (row < 64u) {{
-                    *reinterpret_cast<u32*>(kb + row * DP + c0) = codes_of(xk[it], s_k, ik, upk);
+                    kt[key_at(row, c0) >> 2] = codes_of(xk[it], s_k, ik, upk);
                     const u32 cv = codes_of(xv[it], s_v, iv, upv);
                     #pragma unroll
-                    for (u32 c = 0; c < 4u; ++c) vt8[(c0 + c) * 68u + row] = (unsigned char)(cv >> (8u * c));
+                    for (u32 c = 0; c < 4u; ++c) vt8[value_at(row, c0 + c)] = (unsigned char)(cv >> (8u * c));
                 }}
             }}
             __syncthreads();
-            u32* __restrict__ vb = reinterpret_cast<u32*>(vc + at * (64u * DP));
-            for (u32 i = t; i < DP * 16u; i += {NT}u) vb[i] = vt[(i >> 4) * 17u + (i & 15u)];
+            uint4* __restrict__ kb = reinterpret_cast<uint4*>(kc + at * (64u * DP));
+            uint4* __restrict__ vb = reinterpret_cast<uint4*>(vc + at * (64u * DP));
+            for (u32 i = t; i < DP * 8u; i += {NT}u) {{
+                if (i < DP * 4u) kb[i] = reinterpret_cast<const uint4*>(kt)[i];
+                else vb[i - DP * 4u] = reinterpret_cast<const uint4*>(vt)[i - DP * 4u];
+            }}
         }}
         __syncthreads();
     }}
@@ -436,25 +454,26 @@ def cache8_read_kernel(DP: int) -> tuple[str, str, str]:
     """The values that the cache of one layer stands for, as fp32 k and v (B, N, H * d): code * scale for the tokens of full
     blocks, the rows themselves for those of the tail, zeros from position lengths[b] + counts[b] on (counts: rows written
     since the lengths were advanced; `extra` for every sequence without them).  One workgroup per (block of 64, head,
-    sequence); value codes are transposed through LDS so that rows leave as rows.  Bound by memory."""
+    sequence); the codes pass through LDS so that rows leave as rows.  Bound by memory."""
     name = f"cache8_read_d{DP}"
-    src = f"""{PRELUDE}{_CACHE8}
-#define DP {DP}u
-extern "C" __global__ __launch_bounds__(256) void {name}(const unsigned char* __restrict__ kc, const unsigned char* __restrict__ vc,
+    src = f"""{PRELUDE}{_CACHE8}{_cache8_layout(DP)}extern "C" __global__ __launch_bounds__(256) void {name}(const unsigned char* __restrict__ kc, const unsigned char* __restrict__ vc,
         const float* __restrict__ scales, const float* __restrict__ tail_k, const float* __restrict__ tail_v,
         const float* __restrict__ lengths, const float* __restrict__ counts, float* __restrict__ ko, float* __restrict__ vo,
         u32 N, u32 H, u32 d, u32 NB, u32 extra) {{
-    __shared__ __attribute__((aligned(16))) u32 vt[DP * 17u];               // rows of 64 bytes, 68 apart
+    __shared__ __attribute__((aligned(16))) u32 kt[DP * 16u], vt[DP * 16u];       // the block's bytes
     const u32 t = threadIdx.x, blk = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
     u32 len, n;
     cache8_extent(lengths, counts, b, extra, NB * 64u, len, n);
     const u32 total = len + n, last = total >> 6;
     const u64 bh = (u64)b * H + h, heads = (u64)gridDim.z * H, at = bh * NB + blk;
     const float s_k = blk < last ? scales[2u * at] : 0.0f, s_v = blk < last ? scales[2u * at + 1u] : 0.0f;
-    const unsigned char* __restrict__ kb = kc + at * (64u * DP);
     if (blk < last) {{
-        const u32* __restrict__ vb = reinterpret_cast<const u32*>(vc + at * (64u * DP));
-        for (u32 i = t; i < DP * 16u; i += 256u) vt[(i >> 4) * 17u + (i & 15u)] = vb[i];
+        const uint4* __restrict__ kb = reinterpret_cast<const uint4*>(kc + at * (64u * DP));
+        const uint4* __restrict__ vb = reinterpret_cast<const uint4*>(vc + at * (64u * DP));
+        for (u32 i = t; i < DP * 8u; i += 256u) {{
+            if (i < DP * 4u) reinterpret_cast<uint4*>(kt)[i] = kb[i];
+            else reinterpret_cast<uint4*>(vt)[i - DP * 4u] = vb[i - DP * 4u];
+        }}
     }}
     __syncthreads();
     const float* __restrict__ tk = tail_k + (((u64)(blk & 1u) * heads + bh) * 64u) * DP;
@@ -466,11 +485,11 @@ extern "C" __global__ __launch_bounds__(256) void {name}(const unsigned char* __
         if (p >= N || c >= d) continue;
         float4 x = make_float4(0.f, 0.f, 0.f, 0.f), z = x;
         if (blk < last) {{
-            const u32 w = *reinterpret_cast<const u32*>(kb + row * DP + c);
-            const unsigned char* vt8 = reinterpret_cast<const unsigned char*>(vt) + c * 68u + row;
+            const u32 w = kt[key_at(row, c) >> 2];
+            const unsigned char* vt8 = reinterpret_cast<const unsigned char*>(vt) + value_at(row, c);             // (four columns of one tile: 16 apart)
             x = make_float4((float)((int)(w & 255u) - 128) * s_k, (float)((int)((w >> 8) & 255u) - 128) * s_k,
                             (float)((int)((w >> 16) & 255u) - 128) * s_k, (float)((int)(w >> 24) - 128) * s_k);
-            z = make_float4((float)((int)vt8[0] - 128) * s_v, (float)((int)vt8[68] - 128) * s_v, (float)((int)vt8[136] - 128) * s_v, (float)((int)vt8[204] - 128) * s_v);
+            z = make_float4((float)((int)vt8[0] - 128) * s_v, (float)((int)vt8[16] - 128) * s_v, (float)((int)vt8[32] - 128) * s_v, (float)((int)vt8[48] - 128) * s_v);
         }} else if (p < total) {{
             x = *reinterpret_cast<const float4*>(tk + row * DP + c);
             z = *reinterpret_cast<const float4*>(tv + row * DP + c);
@@ -507,8 +526,8 @@ def cache8_attend_kernel(DP: int, NQ: int = 1, W: int = 4, stream: bool = False)
     A wavefront takes one block of 64 tokens at a time, for NQ tiles of 16 query rows, with (m, l, O) of its own.  Its lane
     r + 16 g (r < 16, g < 4) holds query r of each tile and, of every product S^T, four tokens; the rows of K are fed in the order
     that makes those of the four token tiles the sixteen neighbours 16 g ..: then P is already the B operand of O^T += V^T P^T,
-    and its A operand, sixteen value codes of one column, is one 16-byte load from the transposed block.  Nothing passes through
-    LDS.  Bytes become 16-bit floats in one operation each: v_perm puts byte c under the exponent of 1024, giving 1024 + c, and
+    and its A operand, sixteen value codes of one column, one 16-byte load.  Nothing passes through
+    LDS, and each load is one run of memory (_cache8_layout).  Bytes become 16-bit floats in one operation each: v_perm puts byte c under the exponent of 1024, giving 1024 + c, and
     a packed addition takes 1152 away.  The keys of the next block are loaded when those of this one have been used, while its
     softmax runs, and its values likewise during the next scores.  stream: loads that leave no trace in the caches, for codes that
     are read once and would only displace others.
@@ -521,14 +540,15 @@ def cache8_attend_kernel(DP: int, NQ: int = 1, W: int = 4, stream: bool = False)
     the vector units: about 2 operations per score and code against a matrix instruction's 1/16."""
     ND, NK, Q4 = DP // 16, DP // 32, DP // 4             # column tiles of V^T, k steps of a score, columns a lane feeds
     name = f"cache8_attend_d{DP}" + (f"_q{NQ}" if NQ > 1 else "") + (f"_w{W}" if W != 4 else "") + ("_nt" if stream else "")
+    wide = Q4 % 16 == 0                                   # a lane's quarter of a key in 16-byte words, else in words of 8
+    kw, kn = (Q4 // 16, 4) if wide else (Q4 // 8, 2)
     fetch = "__builtin_nontemporal_load({})" if stream else "*{}"
-    fetch2, fetch4 = (fetch.format(f"reinterpret_cast<const u{n}*>({at})") for n, at in ((2, "p + 4u * u * DP + 8u * i"), (4, "p + dt * 1024u")))
-    kw = Q4 // 8                                          # 8-byte words of a key row per lane
+    fetch_k = fetch.format(f"reinterpret_cast<const u{kn}*>(p + u * {64 * Q4}u + i * {256 * kn}u)")
+    fetch_v = fetch.format("reinterpret_cast<const u4*>(p + dt * 1024u)")
+    half = ("i & 1u ? kr[u][i >> 1].z : kr[u][i >> 1].x, i & 1u ? kr[u][i >> 1].w : kr[u][i >> 1].y" if wide else "kr[u][i].x, kr[u][i].y")
     # "256, 2" holds the kernel to 256 registers, with which the matrix instructions write ordinary ones; wider heads need more
     bounds = "256, 2" if W == 4 and DP * NQ <= 128 else f"{64 * W}"
-    src = f"""{PRELUDE}{_CACHE8}
-#define DP {DP}u
-#define ND {ND}u
+    src = f"""{PRELUDE}{_CACHE8}{_cache8_layout(DP)}#define ND {ND}u
 #define NK {NK}u
 #define NQ {NQ}u
 #define W {W}u
@@ -627,28 +647,34 @@ extern "C" __global__ __launch_bounds__({bounds}) void {name}(const float* __res
     const u32 nb = min(last, (most + 63u) >> 6);                                    // blocks of codes that the tiles see
     const u32 j0 = (u32)((u64)nb * split / splits) + w, j1 = (u32)((u64)nb * (split + 1u) / splits);
     const u64 base = ((u64)bh * NB) * (64u * DP);
-    const unsigned char* __restrict__ kh = kc + base + (16u * (r >> 2) + (r & 3u)) * DP + g * {Q4}u;     // + 4 u DP for token tile u
-    const unsigned char* __restrict__ vh = vc + base + r * 64u + g * 16u;                              // + 1024 dt for column tile dt
+    const unsigned char* __restrict__ kh = kc + base + lane * {4 * kn}u;
+    const unsigned char* __restrict__ vh = vc + base + lane * 16u;
     const float2* __restrict__ sh = reinterpret_cast<const float2*>(scales) + (u64)bh * NB;
-    u2 kr[4][{kw}];
+    u{kn} kr[4][{kw}];
     u4 vr[ND];
-    float2 sc;
+    // lane i keeps the scales of this wavefront's i-th block, 64 blocks at a time: none is waited for inside a block
+    float2 sc = make_float2(0.0f, 0.0f);
     auto load_k = [&](u32 j) {{
         const unsigned char* __restrict__ p = kh + (u64)j * (64u * DP);
         #pragma unroll
         for (u32 u = 0; u < 4u; ++u)
             #pragma unroll
-            for (u32 i = 0; i < {kw}u; ++i) kr[u][i] = {fetch2};
+            for (u32 i = 0; i < {kw}u; ++i) kr[u][i] = {fetch_k};
     }};
     auto load_v = [&](u32 j) {{
         const unsigned char* __restrict__ p = vh + (u64)j * (64u * DP);
         #pragma unroll
-        for (u32 dt = 0; dt < ND; ++dt) vr[dt] = {fetch4};
+        for (u32 dt = 0; dt < ND; ++dt) vr[dt] = {fetch_v};
     }};
-    if (j0 < j1) {{ load_k(j0); sc = sh[j0]; load_v(j0); }}
+    if (j0 < j1) {{ load_k(j0); load_v(j0); }}
     auto block = [&](u32 j, auto kind) {{
         constexpr bool edge = decltype(kind)::edge;                                 // some query does not see all of the block
-        const u32 jn = j + W < j1 ? j + W : j;                                     // (the last one is loaded again)
+        const u32 jn = j + W < j1 ? j + W : j, nth = ((j - j0) / W) & 63u;             // (the last one is loaded again)
+        if (nth == 0u) {{
+            sc = sh[min(j + W * lane, j1 - 1u)];
+            asm volatile("" : "+v"(sc.x), "+v"(sc.y));                              // (waited for here, not by every block)
+        }}
+        const float ks = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(sc.x), nth)), vs0 = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(sc.y), nth));
         f4 s[NQ][4];
         #pragma unroll
         for (u32 u = 0; u < 4u; ++u) {{
@@ -656,7 +682,7 @@ extern "C" __global__ __launch_bounds__({bounds}) void {name}(const float* __res
             for (u32 a = 0; a < NQ; ++a) s[a][u] = (f4){{0.f, 0.f, 0.f, 0.f}};
             #pragma unroll
             for (u32 i = 0; i < NK; ++i) {{
-                const h8 k8 = widen(kr[u][i].x, kr[u][i].y);
+                const h8 k8 = widen({half});
                 #pragma unroll
                 for (u32 a = 0; a < NQ; ++a) {{
                     s[a][u] = MFMA16(k8, q2[a][i].v, s[a][u]);
@@ -664,11 +690,9 @@ extern "C" __global__ __launch_bounds__({bounds}) void {name}(const float* __res
                 }}
             }}
         }}
-        const float2 now = sc;
         load_k(jn);
-        sc = sh[jn];
         const u32 at = j * 64u + 16u * g;
-        const float vs = now.y == now.y ? now.y : 0.0f;                            // (a NaN scale makes the scores NaN as well)
+        const float vs = vs0 == vs0 ? vs0 : 0.0f;                           // (a NaN scale makes the scores NaN as well)
         H8 p1[NQ][2], p2[NQ][2];
         #pragma unroll
         for (u32 a = 0; a < NQ; ++a) {{
@@ -680,7 +704,7 @@ extern "C" __global__ __launch_bounds__({bounds}) void {name}(const float* __res
             #pragma unroll
             for (u32 i = 1; i < 16u; ++i) mx = fmaxf(mx, s[a][i >> 2][i & 3u]);
             mx = four_max(mx);
-            const float f = back[a] * now.x;                                        // not negative: the maximum stays one
+            const float f = back[a] * ks;                                        // not negative: the maximum stays one
             const float mn = fmaxf(m[a], mx * f), mu = mn == NINF ? 0.0f : mn;
             if (__any(mn != m[a])) {{                                               // (a maximum that stays is the rule after the first blocks)
                 const float alpha = __builtin_amdgcn_exp2f(m[a] - mu);

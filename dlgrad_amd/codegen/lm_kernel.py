@@ -532,7 +532,7 @@ def cache8_attend_kernel(DP: int, NQ: int = 1, W: int = 4, stream: bool = False)
     softmax runs, and its values likewise during the next scores.  stream: loads that leave no trace in the caches, for codes that
     are read once and would only displace others.
 
-    The tail, fp32, is shared out 16 tokens to a wavefront and goes through v_mfma_f32_16x16x4_f32.
+    The tail, fp32, is shared out 16 tokens to a wavefront and goes through v_mfma_f32_16x16x4_f32, with q1 + q2 as the query.
 
     A workgroup of W wavefronts per (NQ tiles of one key head, split of the blocks); they are joined through LDS in
     wavefront order.  With one split y is written; else O, m and l go to `part` and cache8_join_kernel adds the splits up
@@ -593,7 +593,7 @@ struct Edge {{ static constexpr bool edge = true; }};
 extern "C" __global__ __launch_bounds__({bounds}) void {name}(const float* __restrict__ q, const unsigned char* __restrict__ kc,
         const unsigned char* __restrict__ vc, const float* __restrict__ scales, const float* __restrict__ tail_k, const float* __restrict__ tail_v,
         const float* __restrict__ lengths, const float* __restrict__ counts, float* __restrict__ y, float* __restrict__ part,
-        u32 B, u32 T, u32 H, u32 group, u32 d, u32 NB, u32 tiles, u32 splits, float scale) {{
+        u32 B, u32 T, u32 H, u32 group, u32 d, u32 NB, u32 tiles, u32 splits, u32 q_wide, float scale) {{
     __shared__ float so[W][16][DP + 4u];
     __shared__ float sm[W][16], sl[W][16];
     const u32 t = threadIdx.x, w = __builtin_amdgcn_readfirstlane(t >> 6), lane = t & 63u, r = lane & 15u, g = lane >> 4;
@@ -615,20 +615,31 @@ extern "C" __global__ __launch_bounds__({bounds}) void {name}(const float* __res
     H8 q1[NQ][NK], q2[NQ][NK];
     float back[NQ];
     u32 see[NQ];                                                              // positions this lane's queries see
-    const float* qrow[NQ];
     #pragma unroll
     for (u32 a = 0; a < NQ; ++a) {{
         const u32 row = row0 + 16u * a + r, tq = row / group;
         const bool live = row < rows && tq < n;
         see[a] = live ? len + tq + 1u : 0u;
-        qrow[a] = q + ((u64)b * T + (live ? tq : 0u)) * C + (u64)(h * group + row % group) * d;
+        const float* __restrict__ qrow = q + ((u64)b * T + (live ? tq : 0u)) * C + (u64)(h * group + row % group) * d;
         float f[{Q4}], mx = 0.0f;
-        #pragma unroll
-        for (u32 i = 0; i < {Q4}u; ++i) {{
-            const u32 c = g * {Q4}u + i;
-            f[i] = (live && c < d) ? qrow[a][c] : 0.0f;
-            mx = fmaxf(mx, fabsf(f[i]));
+        if (q_wide) {{                                                        // rows of whole 16-byte items
+            #pragma unroll
+            for (u32 i = 0; i < {Q4 // 4}u; ++i) {{
+                const u32 c = g * {Q4}u + 4u * i;
+                const float4 x = *reinterpret_cast<const float4*>(qrow + min(c, d - 4u));
+                const bool in = live && c < d;
+                f[4u * i] = in ? x.x : 0.0f; f[4u * i + 1u] = in ? x.y : 0.0f; f[4u * i + 2u] = in ? x.z : 0.0f; f[4u * i + 3u] = in ? x.w : 0.0f;
+            }}
+        }} else {{
+            #pragma unroll
+            for (u32 i = 0; i < {Q4}u; ++i) {{
+                const u32 c = g * {Q4}u + i;
+                const float x = qrow[min(c, d - 1u)];
+                f[i] = live && c < d ? x : 0.0f;
+            }}
         }}
+        #pragma unroll
+        for (u32 i = 0; i < {Q4}u; ++i) mx = fmaxf(mx, fabsf(f[i]));
         mx = four_max(mx);
         const int e = max((int)((__float_as_uint(mx) >> 23) & 255u), 27) - 127;      // 2^e <= mx < 2^(e + 1)
         const float up = copysignf(__uint_as_float((u32)(14 - e + 127) << 23), scale);
@@ -760,14 +771,11 @@ extern "C" __global__ __launch_bounds__({bounds}) void {name}(const float* __res
         for (u32 a = 0; a < NQ; ++a) {{
             f4 acc = (f4){{0.f, 0.f, 0.f, 0.f}};
             #pragma unroll
-            for (u32 i = 0; i < {Q4}u; ++i) {{
-                const u32 c = g * {Q4}u + i;
-                acc = MFMA32(kt[i], (see[a] && c < d) ? qrow[a][c] : 0.0f, acc);
-            }}
+            for (u32 i = 0; i < {Q4}u; ++i) acc = MFMA32(kt[i], (float)q1[a][i >> 3].e[i & 7u] + (float)q2[a][i >> 3].e[i & 7u], acc);
             float mx = NINF;
             #pragma unroll
             for (u32 i = 0; i < 4u; ++i) {{
-                acc[i] = p0 + i < see[a] ? acc[i] * (scale * 1.44269504088896340736f) : NINF;
+                acc[i] = p0 + i < see[a] ? acc[i] * back[a] : NINF;
                 mx = fmaxf(mx, acc[i]);
             }}
             mx = four_max(mx);
@@ -820,7 +828,7 @@ extern "C" __global__ __launch_bounds__({bounds}) void {name}(const float* __res
     }}
 }}
 """
-    return src, name, _fmt("P" * 10, "I" * 8, "f")
+    return src, name, _fmt("P" * 10, "I" * 9, "f")
 
 
 CACHE8_MAX_SPLITS = 64      # what one wavefront joins: a lane per split

@@ -168,9 +168,9 @@ class Rotary:
         if len({(x.shape[0], s[1]) for x, s in zip(xs, shapes)}) > 1:
             raise ValueError(f"rotary: {' and '.join(str(x.shape) for x in xs)} have different sequences")
         B, T = x.shape[0], shapes[0][1]
-        if positions is not None and positions.numel not in (T, B * T):
+        if positions is not None and positions.shape not in ((T,), (1, T), (B, T)):
             raise ValueError(f"rotary: positions {positions.shape} for {B} sequences of {T}")
-        if start is not None and start.numel not in (1, B):
+        if start is not None and start.numel != 1 and start.shape not in ((B,), (B, 1)):
             raise ValueError(f"rotary: starts {start.shape} for {B} sequences")
         return shapes
 
@@ -227,9 +227,10 @@ class QuantizedKVCache:
     lengths (B, 1), tokens held per sequence, is a device tensor (one of the caller's if given), so a captured step works at
     any length.  counts (B, 1): how many of the T rows of each sequence are tokens (a padded batch); the rest is neither
     written nor seen, and their rows of the result are zeros.  Rows that do not fit into the capacity (rounded up to whole blocks) are
-    dropped the same way.  Until advance() a write may be repeated or replaced, and advance() may be given less than
-    was written if that was at most 64 rows.  A row with a NaN or an infinity makes every result that sees its block, once
-    that is full, or itself, before, NaN.  Results carry no tape.
+    dropped the same way.  Until advance(), a write of at most 64 rows may be repeated or replaced, and advance() may be given
+    less than was written; a longer one can be repeated where every sequence holds whole blocks.  A row with a NaN or an
+    infinity makes every result that sees its block, once that is full, or itself, before, NaN.  Values are to stay below 2^88 in
+    magnitude.  Results carry no tape.
 
     Query heads share key heads in order: query heads h * G .. h * G + G - 1 read key head h, G = n_head / n_kv_head."""
 
@@ -350,7 +351,7 @@ def adjust_logits(logits: Tensor, history: Tensor | None = None, lengths: Tensor
 
     history (B, L): token ids said so far, the first lengths[b] of each row (all without lengths); ids outside [0, V) count for
     nothing.  A token that occurs c > 0 times there becomes x / repetition if x > 0 and x * repetition otherwise, less
-    presence + frequency * c; the three are numbers, or tensors with one per row.  Then bias (V,) or (B, V) is added, and
+    presence + frequency * c; the three are numbers, or tensors with one per row (taken as they are).  Then bias (V,) or (B, V) is added, and
     tokens that hidden (V,) or (B, V) marks (> 0: a grammar's mask) become -inf whatever they were; a row may be hidden
     whole.  One launch on the hip device; elsewhere on the host, from the downloaded logits."""
     _no_tape("adjust_logits", logits, bias)

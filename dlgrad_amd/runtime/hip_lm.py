@@ -242,15 +242,16 @@ class HIPLM:
         k, join = kernel(K.cache8_attend_kernel, c.width, nq, waves, HIPLM.attend_streams(c, tiles)), kernel(K.cache8_join_kernel, c.width) if splits > 1 else None
         held = (c.kc.addr, c.vc.addr, _addr(c.scales), _addr(c.tail_k), _addr(c.tail_v))
         sizes = (c.batch, T, c.heads, group, c.d, c.blocks, tiles, splits)
+        wide = c.d % 4 == 0                                              # (then the rows of the queries are whole 16-byte items)
         n_part, join_grid, join_sizes = pairs * rows * splits * (c.width + 2), (pairs * rows + 3) // 4, (pairs * rows, T, c.heads, group, c.d, splits)
 
         def run(qa: int, la: int, ca: int, scale: float) -> DevicePtr:
             y = alloc(numel)
             if join is None:
-                launch(k, grid, 64 * waves, qa, *held, la, ca, y.addr, 0, *sizes, scale)
+                launch(k, grid, 64 * waves, qa, *held, la, ca, y.addr, 0, *sizes, int(wide and not qa & 15), scale)
                 return y
             part = alloc(n_part)
-            launch(k, grid, 64 * waves, qa, *held, la, ca, y.addr, part.addr, *sizes, scale)
+            launch(k, grid, 64 * waves, qa, *held, la, ca, y.addr, part.addr, *sizes, int(wide and not qa & 15), scale)
             launch(join, join_grid, 256, part.addr, y.addr, *join_sizes)
             return y
         return run

@@ -245,6 +245,7 @@ def test_rotary_refusals():
     x = Tensor(np.zeros((2, 3, 16), f32))
     for call in (lambda: rope(x, 3), lambda: rope(x, 0), lambda: rope(Tensor(np.zeros((2, 2, 3, 16), f32)), 1), lambda: rope(Tensor(np.zeros((3, 16), f32)), 2),
                  lambda: rope(x, 2, positions=Tensor(np.zeros((2, 2), f32))), lambda: rope(x, 2, start=Tensor(np.zeros((3, 1), f32))),
+                 lambda: rope(x, 2, positions=Tensor(np.zeros((3, 2), f32))),
                  lambda: rope.pair(x, Tensor(np.zeros((2, 4, 16), f32)), 2), lambda: rope.pair(x, Tensor(np.zeros((1, 3, 16), f32)), 2)):
         with pytest.raises(ValueError):
             call()
@@ -580,6 +581,44 @@ def test_cache_attention_of_extreme_queries():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("scale", [-0.3, 0.0, 1e-30, 4.0])
+def test_cache_attention_with_any_scale(scale):
+    require_gpu()
+    rng = np.random.default_rng(18)
+    n, d = 150, 64
+    k, v = rows_of(rng, 1, n, d)
+    cache = filled(1, 192, 1, d, (k[:, :-1], v[:, :-1]))
+    cache.write(hip_tensor(k[:, -1:]), hip_tensor(v[:, -1:]))
+    kk, vv = (held(a[0].reshape(n, 1, d), n // BLOCK * BLOCK) for a in (k, v))
+    q = rng.standard_normal((1, 1, 2 * d)).astype(f32)
+    want, tol = attended(q.reshape(1, 2, d), kk, vv, n - 1, scale, 1)
+    if scale < 0:
+        tol = attended(q.reshape(1, 2, d), -kk, vv, n - 1, -scale, 1)[1]       # the same scores, a bound of the right sign
+    within(cache.attend(hip_tensor(q), scale).numpy().reshape(1, 2, d), want, tol)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d", [64, 40])
+def test_cache_of_unaligned_views(d):
+    """Queries, keys and values four bytes off a 16-byte boundary: the same bits."""
+    require_gpu()
+    rng = np.random.default_rng(19)
+    k, v = rows_of(rng, 2, 70, 2 * d)
+    q = rng.standard_normal((2, 70, 4 * d)).astype(f32)
+
+    def off(a):
+        room = Buffer.from_numpy(np.concatenate([np.zeros(1, f32), a.reshape(-1)]), Device.HIP)
+        return Tensor(Buffer(room.ptr + 1, a.shape, Device.HIP))
+    got = []
+    for make in (hip_tensor, off):
+        cache = nn.QuantizedKVCache(2, 128, 2, d)
+        cache.write(make(k), make(v))
+        got.append([cache.attend(make(q)).numpy(), *[t.numpy() for t in cache.read(70, new=70)]])
+    for a, b in zip(*got):
+        same(a, b)
+
+
+@pytest.mark.gpu
 def test_cache_padding_and_empty_sequences():
     """Rows beyond counts give zeros and are not seen; a sequence without tokens gives zeros."""
     require_gpu()
@@ -859,6 +898,41 @@ def test_rotary_gpt_trains_as_on_the_cpu(T):
     assert abs(got["hip"][0] - got["cpu"][0]) <= 1e-4 * abs(got["cpu"][0])
     for name, want in got["cpu"][1].items():
         assert np.abs(got["hip"][1][name] - want).max() <= 1e-4 * np.abs(want).max(), name
+
+
+@pytest.mark.gpu
+def test_rotary_gpt_steps_in_a_captured_graph():
+    """Forward, backward and the optimizer's step recorded once: every replay leaves the weights of an eager step, bit for bit."""
+    require_gpu()
+    if hip.COMPILE_ONLY:
+        return
+    rng = np.random.default_rng(8)
+    ids, targets = (rng.integers(0, 33, (3, 96)).astype(f32) for _ in range(2))
+    weights = []
+    for captured in (False, True):
+        model = gpt("hip", positions="rotary", std=0.05)
+        opt = nn.optim.Adam(nn.utils.get_parameters(model), lr=1e-3)
+        it, tt = hip_tensor(ids), hip_tensor(targets)
+
+        def step():
+            for p in nn.utils.get_parameters(model):
+                p.grad = None
+            _, loss = model(it, tt)
+            loss.backward()
+            opt.step()
+            return loss
+        run = hip.CapturedStep(step, before_replay=opt.advance) if captured else step
+        losses = []
+        for i in range(6):
+            losses.append(float(run().numpy()))
+            if i == 3:
+                nn.adjust_logits(hip_tensor(rng.standard_normal((2, 9)))).numpy()         # work of its own between the replays
+        weights.append((losses, [p.numpy() for p in nn.utils.get_parameters(model)]))
+        if captured:
+            run.close()
+    assert weights[0][0] == weights[1][0]
+    for a, b in zip(weights[0][1], weights[1][1]):
+        same(a, b)
 
 
 @pytest.mark.gpu

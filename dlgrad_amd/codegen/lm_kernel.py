@@ -287,8 +287,11 @@ static __device__ __forceinline__ u32 value_at(u32 row, u32 c) {{ return (c >> 4
 """
 
 
+CACHE8_WRITE_THREADS = 512
+
+
 @cache
-def cache8_write_kernel(DP: int, vec: bool, NT: int = 1024) -> tuple[str, str, str]:
+def cache8_write_kernel(DP: int, vec: bool) -> tuple[str, str, str]:
     """New key and value rows k, v (B, T, H * d) into the 8-bit cache of one layer, at positions lengths[b] .. of each sequence
     (the first counts[b] rows of each, all T without counts; rows that the cache has no room for are dropped).
 
@@ -304,10 +307,13 @@ def cache8_write_kernel(DP: int, vec: bool, NT: int = 1024) -> tuple[str, str, s
     A row that holds a NaN or an infinity is kept as NaN in the tail, and a block with such a row gets NaN for its scales:
     every output that sees it is NaN, and the codes stay whole numbers.
 
-    One workgroup of NT threads per (block of 64, head, sequence), a thread per four columns of a row (16 DP / NT times).  Workgroup 0 of a head completes the block that the call starts in and then stores
+    One workgroup of 512 threads per (block of 64, head, sequence), a thread per four columns of a row (DP / 32 times).  With 256 a
+    launch of few workgroups, which is one pass over the code, takes longer (2 x 12 heads of 64, 512 tokens: 6.7 us against 5.4),
+    with 1024 many wait for each other's barriers (4 x 12 heads of 64, 4096 tokens: 37 us against 29, 4.4 TB/s).  Workgroup 0 of a head completes the block that the call starts in and then stores
     the rows of the block it ends in, in this order, because both may use the same tail.  Bound by memory for long calls: 4 bytes
     read and 1 written per element."""
-    name = f"cache8_write_d{DP}_{'v4' if vec else 'v1'}_t{NT}"
+    name = f"cache8_write_d{DP}_{'v4' if vec else 'v1'}"
+    NT = CACHE8_WRITE_THREADS
     IT = -(-16 * DP // NT)                     # four columns of a row per thread, so many times
     if vec:
         # one load whatever the row is: a choice between two loads would wait for one before the other

@@ -146,13 +146,6 @@ class HIPLM:
             raise ValueError(f"{what}: {lengths.numel} lengths and {'no' if counts is None else counts.numel} counts for {c.batch} sequences")
 
     @staticmethod
-    def write_threads(workgroups: int, compute_units: int) -> int:
-        """Threads per block of 64 tokens that the write takes.  A launch of few workgroups is one pass over the code, shorter with fewer
-        elements a thread (1 x 8 heads of 128, 512 tokens: 12.1 us with 256, 8.3 with 512, 7.2 with 1024); many small ones hide
-        each other's barriers (8 x 12 heads of 64, 1024 tokens: 20.4, 17.5, 20.4 us; 4 x 12 x 4096: 37.2, 32.5, 40.7)."""
-        return 1024 if workgroups <= 2 * compute_units else 512
-
-    @staticmethod
     def cache8_writer(c: Cache8, shape: tuple):
         """The checks of cache8_write that depend on the shape of the keys alone, and run(addresses of keys, values, lengths, counts)."""
         C = c.heads * c.d
@@ -161,7 +154,6 @@ class HIPLM:
         T = shape[1]
         if T > c.blocks * K.CACHE8_BLOCK:
             raise ValueError(f"cache8_write: {T} tokens for a cache of {c.blocks * K.CACHE8_BLOCK}")
-        NT = HIPLM.write_threads(-(-T // K.CACHE8_BLOCK) * c.heads * c.batch, props()["compute_units"])
         grid, wide, kernels = (-(-T // K.CACHE8_BLOCK), c.heads, c.batch), C % 4 == 0 and c.d % 4 == 0, [None, None]
         tail = (c.kc.addr, c.vc.addr, _addr(c.scales), _addr(c.tail_k), _addr(c.tail_v), T, c.heads, c.d, c.blocks, C, C)
 
@@ -169,9 +161,9 @@ class HIPLM:
             vec = wide and not (ka | va) & 15
             k = kernels[vec]
             if k is None:
-                k = kernels[vec] = kernel(K.cache8_write_kernel, c.width, vec, NT)
+                k = kernels[vec] = kernel(K.cache8_write_kernel, c.width, vec)
             # a call completes at most ceil(T / 64) blocks, the one it starts in among them
-            launch(k, grid, NT, ka, va, la, ca, *tail)
+            launch(k, grid, K.CACHE8_WRITE_THREADS, ka, va, la, ca, *tail)
         return run if T else lambda ka, va, la, ca: None
 
     @staticmethod

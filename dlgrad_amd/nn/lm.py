@@ -308,8 +308,8 @@ class QuantizedKVCache:
             if n.numel != self.batch or n.device is not Device.HIP or n.data.is_host_scalar:
                 raise ValueError(f"advance: counts {n.shape} for {self.batch} sequences")
             step = Tensor(n.data.reshape(self.lengths.shape))
-        elif n < 0:
-            raise ValueError("advance: a cache does not go back; see reset()")
+        elif n < 0 or n != int(n):
+            raise ValueError(f"advance: {n} tokens (a cache does not go back; see reset())")
         else:
             step = float(n)
         self.lengths.data.copy_((self.lengths + step).clamp(max=self.capacity).data)
@@ -351,9 +351,9 @@ def adjust_logits(logits: Tensor, history: Tensor | None = None, lengths: Tensor
 
     history (B, L): token ids said so far, the first lengths[b] of each row (all without lengths); ids outside [0, V) count for
     nothing.  A token that occurs c > 0 times there becomes x / repetition if x > 0 and x * repetition otherwise, less
-    presence + frequency * c; the three are numbers, or tensors with one per row (taken as they are).  Then bias (V,) or (B, V) is added, and
-    tokens that hidden (V,) or (B, V) marks (> 0: a grammar's mask) become -inf whatever they were; a row may be hidden
-    whole.  One launch on the hip device; elsewhere on the host, from the downloaded logits."""
+    presence + frequency * c; the three are numbers, or tensors with one per row (taken as they are).  Then bias, (V,) or
+    (B, V), is added, and tokens that hidden, (V,) or (B, V), marks (> 0: a grammar's mask) become -inf whatever they were; a row
+    may be hidden whole.  One launch on the hip device; elsewhere on the host, from the downloaded logits."""
     _no_tape("adjust_logits", logits, bias)
     given = (logits, history, lengths, repetition, presence, frequency, bias, hidden)
     key = tuple([(t.data.shape, t.data.device, t.data.ptr.__class__) if t.__class__ is Tensor else t for t in given])

@@ -122,7 +122,7 @@ class KVCache8:
 
     def __init__(self, c: GPTConfig, batch: int, lengths: Tensor | None = None) -> None:
         self.store = nn.QuantizedKVCache(batch, c.block_size, c.n_head, c.n_embd // c.n_head, c.n_layer, c.device, lengths)
-        self.batch, self.length = batch, 0
+        self.batch, self.length, self.rows = batch, 0, c.block_size
 
     def start(self) -> Tensor | None:
         return self.store.lengths if self.length else None
@@ -133,6 +133,8 @@ class KVCache8:
 
     def write(self, layer: int, k: Tensor, v: Tensor, at: int) -> None:
         assert at == self.length
+        if at + k.shape[1] > self.rows:
+            raise IndexError(f"positions {at}:{at + k.shape[1]} outside a cache of {self.rows}")
         self.store.write(k, v, layer)
 
 

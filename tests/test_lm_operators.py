@@ -704,6 +704,28 @@ def test_cache_goes_back_over_rows_that_were_not_kept():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("gap", [14, 24, 30, 36])
+def test_cache_attention_adds_up_many_small_weights(gap):
+    """2^20 tokens of weight 2^-gap beside one of weight 1, values around 1: together they move the result by up to 2^(20 - gap)."""
+    require_gpu()
+    rng = np.random.default_rng(gap)
+    n, d = 1 << 20, 32
+    k, v = np.zeros((1, n, d), f32), (1 + 0.25 * rng.standard_normal((1, n, d))).astype(f32)
+    q, last = np.zeros((1, 1, d), f32), rng.standard_normal((1, 1, d)).astype(f32)
+    q[0, 0, 3] = 2.0
+    key = np.zeros((1, 1, d), f32)
+    key[0, 0, 3] = gap * math.log(2) / 2                                  # the score of the last token: gap ln 2
+    cache = filled(1, n + 64, 1, d, (k, v))
+    cache.write(hip_tensor(key), hip_tensor(last))
+    y = cache.attend(hip_tensor(q), 1.0).numpy().reshape(1, 1, d)
+    want, tol = attended(q, np.concatenate([k[0], key[0]])[:, None], np.concatenate([held(v[0][:, None], n), last[0][:, None]]), n, 1.0, 1)
+    # the sums over the tokens: a term is off by 2^-22 of itself, a partial sum by a rounding of the whole
+    small = n * 2.0 ** -gap
+    tol = np.abs(want) * (64 * EPS + 2 * gap * EPS) + small / (1 + small) * (2.0 ** -20 + (64 + n / 64 / 4) * EPS) * np.abs(v).max() + 16 * EPS * np.abs(last).max()
+    within(y, want, tol, f"weights of 2^-{gap}")
+
+
+@pytest.mark.gpu
 def test_cache_beyond_four_gigabytes():
     """Offsets past 32 bits: blocks that were never written have scale 0, so their tokens weigh exp(0) and add nothing."""
     require_gpu()
@@ -803,7 +825,7 @@ def test_cache_refusals():
     for call in (lambda: cache.write(z(2, 1, 64), z(2, 1, 32)), lambda: cache.write(z(1, 1, 64), z(1, 1, 64)), lambda: cache.write(z(2, 64), z(2, 64)),
                  lambda: cache.write(z(2, 65, 64), z(2, 65, 64)), lambda: cache.attend(z(2, 1, 96)), lambda: cache.attend(z(3, 1, 64)),
                  lambda: cache.attend(z(2, 65, 64)), lambda: cache.attend(z(2, 1, 64), counts=z(3, 1)), lambda: cache.read(65), lambda: cache.read(-1),
-                 lambda: cache.advance(-1), lambda: cache.advance(z(3, 1)), lambda: cache.write(Tensor(np.zeros((2, 1, 64), f32)), z(2, 1, 64)),
+                 lambda: cache.advance(-1), lambda: cache.advance(0.5), lambda: cache.advance(z(3, 1)), lambda: cache.write(Tensor(np.zeros((2, 1, 64), f32)), z(2, 1, 64)),
                  lambda: cache.attend(Tensor(np.zeros((2, 1, 64), f32))), lambda: cache.attend(Tensor.full((2, 1, 64), 0.0, device="hip", requires_grad=True)),
                  lambda: cache.attend(z(2, 1, 0))):
         with pytest.raises(ValueError):

@@ -12,9 +12,12 @@ from dlgrad_amd.codegen import lm_kernel as K
 from dlgrad_amd.device import Device
 from dlgrad_amd.dispatch import dispatcher
 from dlgrad_amd.helpers import CustomOps
-from dlgrad_amd.runtime.hip import NT_STORE_MIN_ELEMENTS, DevicePtr, _addr, _PlanCache, _upload, alloc, field_offset, kernel, launch, launch_out, props
+from dlgrad_amd.runtime.hip import DevicePtr, _addr, _PlanCache, _upload, alloc, field_offset, kernel, launch, launch_out, props
 
 STREAM_BYTES = 1 << 28       # the Infinity Cache
+# elements from which rotary positions bypass the L2 caches (queries and keys of 16 x 1024 x 12 heads of 64, 2 x 50 MB: 33.7 us against 39.1, with
+# an addition of the two behind it 59.4 against 62.9; of 8 x 1024, 2 x 25 MB: 17.2 against 18.8, but 17.1 against 16.4 for inputs turned twice)
+ROTARY_STREAM_ELEMENTS = 1 << 23
 EXACT_WHOLE = 1 << 24        # whole numbers up to here are exact in fp32
 _rotary_plans: dict = _PlanCache()     # what a call looked at -> the launch that its checks ended in
 
@@ -93,7 +96,7 @@ class HIPLM:
             if blocks >= 2 ** 31:
                 raise ValueError(f"rotary: {rows} rows exceed the grid")
             return (blocks, 1, 1 + two)
-        stream = not inplace and numel0 + two * numel1 >= NT_STORE_MIN_ELEMENTS
+        stream = not inplace and numel0 + two * numel1 >= ROTARY_STREAM_ELEMENTS
 
         def variant(vec: bool) -> list:
             v = [None, grid(vec), None]

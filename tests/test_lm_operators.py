@@ -165,7 +165,7 @@ def test_rotary_beyond_the_caches_has_the_same_bits(layout, monkeypatch):
     rng = np.random.default_rng(12)
     q, k = rng.standard_normal((2, 33, 6 * 48)).astype(f32), rng.standard_normal((2, 33, 2 * 48)).astype(f32)
     want = [t.numpy() for t in nn.Rotary(48, 32, layout=layout).pair(hip_tensor(q), hip_tensor(k), 6, 2)]
-    monkeypatch.setattr(hip_lm, "NT_STORE_MIN_ELEMENTS", 1)
+    monkeypatch.setattr(hip_lm, "ROTARY_STREAM_ELEMENTS", 1)
     monkeypatch.setattr(hip_lm, "_rotary_plans", {})
     for a, b in zip(nn.Rotary(48, 32, layout=layout).pair(hip_tensor(q), hip_tensor(k), 6, 2), want):
         same(a.numpy(), b)

@@ -65,7 +65,8 @@ def rotary_kernel(half: bool, vec: bool, stream: bool = False) -> tuple[str, str
                 if vec else "const float a = xr[off + j], b = xr[off + hr + j];")
         keep = ("va[n][0] = a.x; va[n][1] = a.y; va[n][2] = a.z; va[n][3] = a.w; vb[n][0] = b.x; vb[n][1] = b.y; vb[n][2] = b.z; vb[n][3] = b.w;"
                 if vec else "va[n][0] = a; vb[n][0] = b;")
-        store = (put("yr + off + j", "oa[0], oa[1], oa[2], oa[3]") + " " + put("yr + off + hr + j", "ob[0], ob[1], ob[2], ob[3]") if vec else "yr[off + j] = oa[0]; yr[off + hr + j] = ob[0];")
+        store = (put("yr + off + j", "oa[0], oa[1], oa[2], oa[3]") + " " + put("yr + off + hr + j", "ob[0], ob[1], ob[2], ob[3]")
+                 if vec else "yr[off + j] = oa[0]; yr[off + hr + j] = ob[0];")
     else:
         load = (f"const float4 a = {get('xr + off + 2u * j')};" if vec
                 else "const float a = xr[off + 2u * j], b = xr[off + 2u * j + 1u];")
@@ -154,7 +155,8 @@ def adjust_logits_kernel(items: int, vec: bool, packed: bool) -> tuple[str, str,
     tokens with integer atomics, whose order does not matter.  So there is one launch, no count array in memory and
     no sort.  packed: two 16-bit counters to a word, for histories of at most 65535 -- half the LDS, twice the blocks on a
     compute unit.  The first 16 entries a thread walks and its logits are loaded before the counters are cleared, so all of
-    these reads are on their way together.  vec: 16-byte accesses (V % 4 == 0)."""
+    these reads are on their way together.  vec: 16-byte accesses (V % 4 == 0).  Bound by memory: 8 bytes a logit (256 x 128256,
+    4000 said: 53.7 us from HBM, 5.0 TB/s; 45 to 47 us partly from the Infinity Cache)."""
     assert items in (4, 8, 16)
     name = f"adjust_logits_i{items}_{'v4' if vec else 'v1'}{'_h' if packed else ''}"
     W = 4 if vec else 1
@@ -309,9 +311,10 @@ def cache8_write_kernel(DP: int, vec: bool) -> tuple[str, str, str]:
 
     One workgroup of 512 threads per (block of 64, head, sequence), a thread per four columns of a row (DP / 32 times).  With 256 a
     launch of few workgroups, which is one pass over the code, takes longer (2 x 12 heads of 64, 512 tokens: 6.7 us against 5.4),
-    with 1024 many wait for each other's barriers (4 x 12 heads of 64, 4096 tokens: 37 us against 29, 4.4 TB/s).  Workgroup 0 of a head completes the block that the call starts in and then stores
-    the rows of the block it ends in, in this order, because both may use the same tail.  Bound by memory for long calls: 4 bytes
-    read and 1 written per element."""
+    with 1024 many wait for each other's barriers (4 x 12 heads of 64, 4096 tokens: 37 us against 29, 4.4 TB/s).  Workgroup 0
+    of a head completes the block that the call starts in and then stores the rows of the block it ends in, in this order,
+    because both may use the same tail.  Bound by memory for long calls, 4 bytes read and 1 written per element; by its chain of
+    reads, reduction and stores for short ones (the token that completes 96 blocks: 5.1 us; one that completes none: 2.7)."""
     name = f"cache8_write_d{DP}_{'v4' if vec else 'v1'}"
     NT = CACHE8_WRITE_THREADS
     IT = -(-16 * DP // NT)                     # four columns of a row per thread, so many times
@@ -460,7 +463,8 @@ def cache8_read_kernel(DP: int) -> tuple[str, str, str]:
     """The values that the cache of one layer stands for, as fp32 k and v (B, N, H * d): code * scale for the tokens of full
     blocks, the rows themselves for those of the tail, zeros from position lengths[b] + counts[b] on (counts: rows written
     since the lengths were advanced; `extra` for every sequence without them).  One workgroup per (block of 64, head,
-    sequence); the codes pass through LDS so that rows leave as rows.  Bound by memory."""
+    sequence); the codes pass through LDS so that rows leave as rows.  Bound by memory (8 x 1024 tokens of 12 heads of 64: 11.3 us,
+    5.6 TB/s)."""
     name = f"cache8_read_d{DP}"
     src = f"""{PRELUDE}{_CACHE8}{_cache8_layout(DP)}extern "C" __global__ __launch_bounds__(256) void {name}(const unsigned char* __restrict__ kc, const unsigned char* __restrict__ vc,
         const float* __restrict__ scales, const float* __restrict__ tail_k, const float* __restrict__ tail_v,
@@ -532,18 +536,20 @@ def cache8_attend_kernel(DP: int, NQ: int = 1, W: int = 4, stream: bool = False)
     A wavefront takes one block of 64 tokens at a time, for NQ tiles of 16 query rows, with (m, l, O) of its own.  Its lane
     r + 16 g (r < 16, g < 4) holds query r of each tile and, of every product S^T, four tokens; the rows of K are fed in the order
     that makes those of the four token tiles the sixteen neighbours 16 g ..: then P is already the B operand of O^T += V^T P^T,
-    and its A operand, sixteen value codes of one column, one 16-byte load.  Nothing passes through
-    LDS, and each load is one run of memory (_cache8_layout).  Bytes become 16-bit floats in one operation each: v_perm puts byte c under the exponent of 1024, giving 1024 + c, and
-    a packed addition takes 1152 away.  The keys of the next block are loaded when those of this one have been used, while its
-    softmax runs, and its values likewise during the next scores.  stream: loads that leave no trace in the caches, for codes that
-    are read once and would only displace others.
+    and its A operand, sixteen value codes of one column, one 16-byte load.  Nothing passes through LDS, and each load is one
+    run of memory (_cache8_layout).  Bytes become 16-bit floats in one operation each: v_perm puts byte c under the exponent
+    of 1024, giving 1024 + c, and a packed addition takes 1152 away.  The keys of the next block are loaded when those of this
+    one have been used, while its softmax runs, and its values likewise during the next scores.  stream: loads that leave no
+    trace in the caches, for codes that are read once and would only displace others.
 
     The tail, fp32, is shared out 16 tokens to a wavefront and goes through v_mfma_f32_16x16x4_f32, with q1 + q2 as the query.
 
     A workgroup of W wavefronts per (NQ tiles of one key head, split of the blocks); they are joined through LDS in
     wavefront order.  With one split y is written; else O, m and l go to `part` and cache8_join_kernel adds the splits up
-    in their order.  Bound by memory while few query rows share a key head: 2 bytes per token and column.  With many, by
-    the vector units: about 2 operations per score and code against a matrix instruction's 1/16."""
+    in their order.  Bound by memory while few query rows share a key head, 2 bytes per token and column (16 sequences up to 32768
+    tokens, 32 heads on 8 of 128: 132 us, 6.2 TB/s); with many by issue, some 290 vector and 32 matrix instructions a block of 64 and
+    tile of 16 rows, which do not overlap (4 x 12 heads of 64, 256 rows after 4096 tokens: 47 us, 285 TFLOP/s of the formula's
+    operations); with few blocks by chains of dependent reads (one block and a tail: 3.9 us)."""
     ND, NK, Q4 = DP // 16, DP // 32, DP // 4             # column tiles of V^T, k steps of a score, columns a lane feeds
     name = f"cache8_attend_d{DP}" + (f"_q{NQ}" if NQ > 1 else "") + (f"_w{W}" if W != 4 else "") + ("_nt" if stream else "")
     wide = Q4 % 16 == 0                                   # a lane's quarter of a key in 16-byte words, else in words of 8
@@ -691,7 +697,8 @@ extern "C" __global__ __launch_bounds__({bounds}) void {name}(const float* __res
             sc = sh[min(j + W * lane, j1 - 1u)];
             asm volatile("" : "+v"(sc.x), "+v"(sc.y));                              // (waited for here, not by every block)
         }}
-        const float ks = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(sc.x), nth)), vs0 = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(sc.y), nth));
+        const float ks = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(sc.x), nth));
+        const float vs0 = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(sc.y), nth));
         f4 s[NQ][4];
         #pragma unroll
         for (u32 u = 0; u < 4u; ++u) {{
@@ -844,7 +851,7 @@ CACHE8_MAX_SPLITS = 64      # what one wavefront joins: a lane per split
 def cache8_join_kernel(DP: int) -> tuple[str, str, str]:
     """Adds up what cache8_attend_kernel left per split: O = sum exp(m_s - M) O_s over sum exp(m_s - M) l_s.  One wavefront per query
     row of a key head: lane s takes m and l of split s (at most 64), the factors go round, and the columns are added in the order of
-    the splits with eight loads in flight.  Bound by latency: two dependent reads."""
+    the splits with eight loads in flight.  Bound by latency: two dependent reads (512 rows of 4 splits: 4.7 us)."""
     name = f"cache8_join_d{DP}"
     N = (DP + 63) // 64
     src = f"""{PRELUDE}

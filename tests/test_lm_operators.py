@@ -839,6 +839,71 @@ def test_cache_refusals():
             nn.QuantizedKVCache(**{**dict(batch=2, capacity=64, n_kv_head=2, head_dim=32), **bad})
 
 
+def test_cache_runtime_refuses_what_does_not_fit():
+    """Host checks of the launches, before any device is touched."""
+    from dlgrad_amd.runtime.hip_lm import Cache8
+
+    class Ptr:
+        addr, nbytes = 256, 1 << 40
+    b = lambda *s: Buffer(Ptr(), s, Device.HIP)                  # noqa: E731
+    c = Cache8.__new__(Cache8)
+    c.batch, c.heads, c.d, c.width, c.blocks, c.layers, c.kc, c.vc = 2, 3, 40, 64, 2, 1, Ptr(), Ptr()
+    c.scales = c.tail_k = c.tail_v = b(1)
+    c.writers, c.attenders = {}, {}
+    for shape in ((2, 1, 121), (1, 1, 120), (2, 120), (2, 129, 120), (2, 1, 1, 120)):
+        with pytest.raises(ValueError):
+            HIPLM.cache8_write(c, b(*shape), b(*shape), b(2))
+    for shape in ((2, 1, 121), (2, 1, 0), (3, 1, 120), (2, 129, 120), (2, 240)):
+        with pytest.raises(ValueError):
+            HIPLM.cache8_attend(c, b(*shape), 1.0, b(2))
+    good = b(2, 1, 120)
+    for call in (lambda: HIPLM.cache8_write(c, good, b(2, 2, 120), b(2)), lambda: HIPLM.cache8_write(c, good, good, b(3)), lambda: HIPLM.cache8_write(c, good, good, b(2), b(1)),
+                 lambda: HIPLM.cache8_write(c, good, Buffer.from_scalar(1.0), b(2)), lambda: HIPLM.cache8_attend(c, good, 1.0, Buffer.from_scalar(1.0)),
+                 lambda: HIPLM.cache8_attend(c, good, 1.0, b(2), b(5)), lambda: HIPLM.cache8_read(c, 129, b(2)), lambda: HIPLM.cache8_read(c, 1, b(2), None, 129),
+                 lambda: HIPLM.cache8_read(c, 1, b(1))):
+        with pytest.raises(ValueError):
+            call()
+    assert HIPLM.cache8_writer(c, (2, 0, 120))(0, 0, 0, 0) is None                # nothing to write: nothing launched
+    assert not c.writers and not c.attenders
+
+
+def test_adjust_logits_runtime_refuses_what_does_not_fit():
+    class Ptr:
+        addr, nbytes = 256, 1 << 40
+    b = lambda *s: Buffer(Ptr(), s, Device.HIP)                  # noqa: E731
+    good = dict(logits=b(4, 10), history=b(4, 3), lengths=b(4), penalties=(1.0, 0.0, 0.0), bias=b(10), hidden=b(4, 10))
+    for bad in (dict(logits=b(40)), dict(logits=b(4, (1 << 24) + 1)), dict(history=b(3, 3)), dict(history=b(12)), dict(history=None), dict(lengths=b(3)),
+                dict(bias=b(4)), dict(hidden=b(2, 10)), dict(hidden=b(4, 10, 1)), dict(penalties=(b(3), 0.0, 0.0)), dict(penalties=(1.0, 0.0, Buffer.from_scalar(2.0))),
+                dict(logits=b(70000, 10), history=b(70000, 3), lengths=None, hidden=None)):
+        with pytest.raises(ValueError):
+            HIPLM.logits_plan(**{**good, **bad})
+
+
+def test_cache_layout_puts_every_byte_in_one_place():
+    """The places of a block's 64 x DP keys and values, restated: a permutation, and what each lane's load is meant to find there."""
+    for DP in (32, 64, 96, 128, 160, 192, 224, 256):
+        Q4 = DP // 4
+        w = 16 if Q4 % 16 == 0 else 8
+        row, c = (a.reshape(-1) for a in np.meshgrid(np.arange(64), np.arange(DP), indexing="ij"))
+        g, i = c // Q4, c % Q4
+        key = ((row >> 2) & 3) * 64 * Q4 + i // w * 64 * w + (g * 16 + ((row >> 4) << 2) + (row & 3)) * w + i % w
+        value = (c >> 4) * 1024 + ((row >> 4) * 16 + (c & 15)) * 16 + (row & 15)
+        for at in (key, value):
+            assert np.array_equal(np.sort(at), np.arange(64 * DP))
+        owner, column = np.empty(64 * DP, int), np.empty(64 * DP, int)
+        owner[key], column[key] = row, c
+        for u in range(4):                                          # lane r + 16 g of token tile u: the g-th quarter of token 16 (r / 4) + 4 u + r % 4
+            for lane in range(64):
+                r, q = lane % 16, lane // 16
+                at = np.concatenate([u * 64 * Q4 + x * 64 * w + lane * w + np.arange(w) for x in range(Q4 // w)])
+                assert (owner[at] == 16 * (r // 4) + 4 * u + r % 4).all() and np.array_equal(column[at], q * Q4 + np.arange(Q4))
+        owner[value], column[value] = row, c
+        for dt in range(DP // 16):                                  # ... and of column tile dt: tokens 16 g .. of column 16 dt + r
+            for lane in range(64):
+                at = dt * 1024 + lane * 16 + np.arange(16)
+                assert np.array_equal(owner[at], 16 * (lane // 16) + np.arange(16)) and (column[at] == 16 * dt + lane % 16).all()
+
+
 def test_cache_is_refused_off_the_device():
     with pytest.raises(ValueError, match="hip device"):
         nn.QuantizedKVCache(1, 64, 1, 32, device="cpu")

@@ -23,9 +23,9 @@ def _result(buf: Buffer) -> Tensor:
     return t
 
 
-def _no_tape(what: str, *tensors) -> None:
-    """Refuses a call whose result would silently stop a gradient."""
-    if any([t.requires_grad for t in tensors if t is not None]) and not _nn._inference_depth:
+def _no_tape(what: str) -> None:
+    """Refuses a call, made with a tensor that requires a gradient, whose result would silently stop that gradient."""
+    if not _nn._inference_depth:
         raise ValueError(f"{what} has no gradient: call it inside nn.inference(), or with detach()ed tensors")
 
 
@@ -270,11 +270,14 @@ class QuantizedKVCache:
     def _sized(self, counts: Tensor | None) -> bool:
         """Whether the lengths and counts of a call are what the launch of an earlier call may read."""
         n = self.lengths.data
-        return n.numel == self.batch and _on_hip(n) and (counts is None or (counts.__class__ is Tensor and counts.data.numel == self.batch and _on_hip(counts.data)))
+        if n.numel != self.batch or n.device is not Device.HIP or n.ptr.__class__ is HostScalar:
+            return False
+        return counts is None or (counts.__class__ is Tensor and counts.data.numel == self.batch and _on_hip(counts.data))
 
     def write(self, k: Tensor, v: Tensor, layer: int = 0, counts: Tensor | None = None) -> None:
         """k, v (B, T, n_kv_head * head_dim): keys and values of positions lengths[b] .. of each sequence."""
-        _no_tape("QuantizedKVCache.write", k, v)
+        if k.requires_grad or v.requires_grad:
+            _no_tape("QuantizedKVCache.write")
         kd, vd = k.data, v.data
         run = self.layers[layer].writers.get(kd.shape) if 0 <= layer < len(self.layers) else None
         if run is not None and kd.shape == vd.shape and _on_hip(kd) and _on_hip(vd) and self._sized(counts):
@@ -285,7 +288,8 @@ class QuantizedKVCache:
     def attend(self, q: Tensor, scale: float | None = None, layer: int = 0, counts: Tensor | None = None) -> Tensor:
         """q (B, T, n_head * head_dim): the queries of positions lengths[b] .., whose keys and values write() has stored; each sees
         the positions up to its own.  scale: of the scores, head_dim ** -0.5 without one."""
-        _no_tape("QuantizedKVCache.attend", q)
+        if q.requires_grad:
+            _no_tape("QuantizedKVCache.attend")
         scale = self.head_dim ** -0.5 if scale is None else float(scale)
         qd = q.data
         run = self.layers[layer].attenders.get(qd.shape) if 0 <= layer < len(self.layers) else None
@@ -319,7 +323,7 @@ class QuantizedKVCache:
         self.lengths.data.copy_(Tensor.full(self.lengths.shape, 0.0, device="hip").data)
 
 
-_adjust_plans: dict = {}       # shapes and numbers that _check_adjust has let through -> the launch (False off the hip device)
+_adjust_plans: dict = {}       # shapes and numbers that _check_adjust has let through -> the launch
 
 
 def _check_adjust(logits, history, lengths, repetition, presence, frequency, bias, hidden) -> None:
@@ -354,22 +358,23 @@ def adjust_logits(logits: Tensor, history: Tensor | None = None, lengths: Tensor
     presence + frequency * c; the three are numbers, or tensors with one per row (taken as they are).  Then bias, (V,) or
     (B, V), is added, and tokens that hidden, (V,) or (B, V), marks (> 0: a grammar's mask) become -inf whatever they were; a row
     may be hidden whole.  One launch on the hip device; elsewhere on the host, from the downloaded logits."""
-    _no_tape("adjust_logits", logits, bias)
-    given = (logits, history, lengths, repetition, presence, frequency, bias, hidden)
-    key = tuple([(t.data.shape, t.data.device, t.data.ptr.__class__) if t.__class__ is Tensor else t for t in given])
-    plan = _adjust_plans.get(key)
-    if plan is None:
-        _check_adjust(*given)
-        args = [t.data if isinstance(t, Tensor) else t for t in given]
-        plan = False                                                    # (checked; not launched from here)
-        if logits.data.device is Device.HIP:
-            from dlgrad_amd.runtime.hip_lm import HIPLM
-            plan = HIPLM.logits_plan(*args[:3], tuple(args[3:6]), *args[6:])
+    if logits.requires_grad or (bias is not None and bias.requires_grad):
+        _no_tape("adjust_logits")
+    x, h, n = logits.data, None if history is None else history.data, None if lengths is None else lengths.data
+    b, m = None if bias is None else bias.data, None if hidden is None else hidden.data
+    r, p, f = (t.data if t.__class__ is Tensor else t for t in (repetition, presence, frequency))
+    given = (h, n, b, m, r, p, f)
+    key = (x.shape, *[(t.shape, t.device, t.ptr.__class__) if isinstance(t, Buffer) else t for t in given])
+    plan = _adjust_plans.get(key) if ops.FUSED and _on_hip(x) else None
+    if plan is not None:
+        return _result(x._like(plan(x, h, n, (r, p, f), b, m)))
+    _check_adjust(logits, history, lengths, repetition, presence, frequency, bias, hidden)
+    if ops.FUSED and logits.device is Device.HIP:
+        from dlgrad_amd.runtime.hip_lm import HIPLM
+        plan = HIPLM.logits_plan(x, h, n, (r, p, f), b, m)
         if len(_adjust_plans) >= 1024:                                  # (a workload whose shapes never repeat)
             _adjust_plans.clear()
         _adjust_plans[key] = plan
-    if plan and ops.FUSED:
-        x, h, n, r, p, f, b, m = [t.data if t.__class__ is Tensor else t for t in given]
         return _result(x._like(plan(x, h, n, (r, p, f), b, m)))
     (B, V), x = logits.shape, logits.numpy().astype(np.float32, copy=True)
     rows = lambda p: p.numpy().reshape(B) if isinstance(p, Tensor) else np.full(B, p, np.float32)      # noqa: E731

@@ -613,17 +613,35 @@ extern "C" __global__ __launch_bounds__({bounds}) void {name}(const float* __res
     const u32 per = tiles * splits, spread = (B * H) % 8u == 0u ? 8u : 1u, at0 = blockIdx.x / spread;
     const u32 bh = (at0 / per) * spread + blockIdx.x % spread, b = bh / H, h = bh % H;
     const u32 split = at0 % splits, tile = (at0 / splits) % tiles;
+    const u32 rows = T * group, row0 = tile * (16u * NQ), row1 = min(row0 + 16u * NQ, rows) - 1u, t0 = row0 / group, t1 = row1 / group;
+    const u64 C = (u64)H * group * d;
+    // this lane's quarter of its query rows: on its way while the lengths are
+    float raw[NQ][{Q4}];
+    #pragma unroll
+    for (u32 a = 0; a < NQ; ++a) {{
+        const u32 row = min(row0 + 16u * a + r, rows - 1u);
+        const float* __restrict__ qrow = q + ((u64)b * T + row / group) * C + (u64)(h * group + row % group) * d;
+        if (q_wide) {{                                                        // rows of whole 16-byte items
+            #pragma unroll
+            for (u32 i = 0; i < {Q4 // 4}u; ++i) *reinterpret_cast<f4*>(&raw[a][4u * i]) = *reinterpret_cast<const f4*>(qrow + min(g * {Q4}u + 4u * i, d - 4u));
+        }} else {{
+            #pragma unroll
+            for (u32 i = 0; i < {Q4}u; ++i) raw[a][i] = qrow[min(g * {Q4}u + i, d - 1u)];
+        }}
+    }}
     u32 len, n;
     cache8_extent(lengths, counts, b, T, NB * 64u, len, n);
-    const u32 rows = T * group, last = (len + n) >> 6;                       // blocks below `last` are codes
-    const u32 row0 = tile * (16u * NQ), row1 = min(row0 + 16u * NQ, rows) - 1u, t0 = row0 / group, t1 = row1 / group;
+    #pragma unroll
+    for (u32 a = 0; a < NQ; ++a)
+        #pragma unroll
+        for (u32 i = 0; i < {Q4}u; ++i) asm volatile("" : "+v"(raw[a][i]));           // (or each would be loaded where it is chosen, one after the other)
+    const u32 last = (len + n) >> 6;                                           // blocks below it are codes
     const u32 most = t0 < n ? len + min(t1, n - 1u) + 1u : 0u;                   // positions that the last query of the tiles sees
     const u32 least = t1 < n ? len + t0 + 1u : 0u;                              // ... and the first (a padded row: none)
-    const u64 C = (u64)H * group * d;
     const float l2 = fabsf(scale) * 1.44269504088896340736f;
     float minus = -1.0f;
     asm volatile("" : "+v"(minus));
-    // this lane's quarter of its query rows, as two 16-bit floats an element; the sign of the scale goes with them
+    // the rows as two 16-bit floats an element; the sign of the scale goes with them
     H8 q1[NQ][NK], q2[NQ][NK];
     float back[NQ];
     u32 see[NQ];                                                              // positions this lane's queries see
@@ -632,26 +650,12 @@ extern "C" __global__ __launch_bounds__({bounds}) void {name}(const float* __res
         const u32 row = row0 + 16u * a + r, tq = row / group;
         const bool live = row < rows && tq < n;
         see[a] = live ? len + tq + 1u : 0u;
-        const float* __restrict__ qrow = q + ((u64)b * T + (live ? tq : 0u)) * C + (u64)(h * group + row % group) * d;
         float f[{Q4}], mx = 0.0f;
-        if (q_wide) {{                                                        // rows of whole 16-byte items
-            #pragma unroll
-            for (u32 i = 0; i < {Q4 // 4}u; ++i) {{
-                const u32 c = g * {Q4}u + 4u * i;
-                const float4 x = *reinterpret_cast<const float4*>(qrow + min(c, d - 4u));
-                const bool in = live && c < d;
-                f[4u * i] = in ? x.x : 0.0f; f[4u * i + 1u] = in ? x.y : 0.0f; f[4u * i + 2u] = in ? x.z : 0.0f; f[4u * i + 3u] = in ? x.w : 0.0f;
-            }}
-        }} else {{
-            #pragma unroll
-            for (u32 i = 0; i < {Q4}u; ++i) {{
-                const u32 c = g * {Q4}u + i;
-                const float x = qrow[min(c, d - 1u)];
-                f[i] = live && c < d ? x : 0.0f;
-            }}
-        }}
         #pragma unroll
-        for (u32 i = 0; i < {Q4}u; ++i) mx = fmaxf(mx, fabsf(f[i]));
+        for (u32 i = 0; i < {Q4}u; ++i) {{
+            f[i] = live && g * {Q4}u + i < d ? raw[a][i] : 0.0f;
+            mx = fmaxf(mx, fabsf(f[i]));
+        }}
         mx = four_max(mx);
         const int e = max((int)((__float_as_uint(mx) >> 23) & 255u), 27) - 127;      // 2^e <= mx < 2^(e + 1)
         const float up = copysignf(__uint_as_float((u32)(14 - e + 127) << 23), scale);

@@ -733,7 +733,9 @@ extern "C" __global__ __launch_bounds__({bounds}) void {name}(const float* __res
             for (u32 i = 1; i < 16u; ++i) mx = fmaxf(mx, s[a][i >> 2][i & 3u]);
             mx = four_max(mx);
             const float f = back[a] * ks;                                        // not negative: the maximum stays one
-            const float mn = fmaxf(m[a], mx * f), mu = mn == NINF ? 0.0f : mn;
+            float top = mx * f;
+            if constexpr (edge) top = j * 64u < see[a] ? top : NINF;                  // (a query that sees none of the block: f may be 0)
+            const float mn = fmaxf(m[a], top), mu = mn == NINF ? 0.0f : mn;
             if (__any(mn != m[a])) {{                                               // (a maximum that stays is the rule after the first blocks)
                 const float alpha = __builtin_amdgcn_exp2f(m[a] - mu);
                 m[a] = mn;

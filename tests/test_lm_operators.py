@@ -726,6 +726,31 @@ def test_cache_attention_adds_up_many_small_weights(gap):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("tiles,waves,splits", [(1, 4, 1), (2, 4, 1), (1, 8, 1), (1, 4, 3)])
+@pytest.mark.parametrize("G,later", [(1, 0.0), (3, 0.0), (1, 1e-36)])
+def test_cache_attention_beside_a_block_of_zero_keys(G, later, tiles, waves, splits, monkeypatch):
+    """Scores far below zero in the first block, keys of nothing (or next to it) in the second: a query that sees none of the second is
+    not moved by its scores, though it shares a tile with queries that do."""
+    require_gpu()
+    monkeypatch.setattr(HIPLM, "attend_tiles", staticmethod(lambda *a: tiles))
+    monkeypatch.setattr(HIPLM, "attend_waves", staticmethod(lambda *a: waves))
+    monkeypatch.setattr(HIPLM, "attend_splits", staticmethod(lambda *a: splits))
+    rng = np.random.default_rng(17)
+    first, T, d = 8, 130, 64
+    n = first + T
+    k, v = rows_of(rng, 1, n, d)
+    k = (-5 + 0.125 * k).astype(f32)                                      # scores around -320: exp of them is nothing in 32 bits
+    k[:, 64:] = later
+    q = np.ones((1, T, G * d), f32)
+    cache = filled(1, n, 1, d, (k[:, :first], v[:, :first]))
+    cache.write(hip_tensor(k[:, first:]), hip_tensor(v[:, first:]))
+    y = cache.attend(hip_tensor(q), 1.0).numpy().reshape(T, G, d)
+    kk, vv = (held(a[0].reshape(n, 1, d), n // 64 * 64) for a in (k, v))
+    want, tol = attended(q[0].reshape(T, G, d), kk, vv, first, 1.0, 1)
+    within(y, want, tol)
+
+
+@pytest.mark.gpu
 def test_cache_beyond_four_gigabytes():
     """Offsets past 32 bits: blocks that were never written have scale 0, so their tokens weigh exp(0) and add nothing."""
     require_gpu()

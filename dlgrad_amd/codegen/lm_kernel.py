@@ -743,11 +743,16 @@ extern "C" __global__ __launch_bounds__({bounds}) void {name}(const float* __res
                 #pragma unroll
                 for (u32 dt = 0; dt < ND; ++dt) o[a][dt] *= alpha;
             }}
-            float sum = 0.0f;
+            float sum = 0.0f, up = 15.0f - mu;
+            if (__any(fabsf(mu) >= 65536.0f)) {{                                     // (roundings of mu could carry p beyond 16-bit floats: first s - mx, exact near 0)
+                up = (top - mu) + 15.0f;
+                #pragma unroll
+                for (u32 i = 0; i < 16u; ++i) s[a][i >> 2][i & 3u] -= mx;
+            }}
             #pragma unroll
             for (u32 i = 0; i < 16u; i += 2u) {{
-                float p = __builtin_amdgcn_exp2f(fmaf(s[a][i >> 2][i & 3u], f, 15.0f - mu));
-                float z = __builtin_amdgcn_exp2f(fmaf(s[a][i >> 2][(i & 3u) + 1u], f, 15.0f - mu));
+                float p = __builtin_amdgcn_exp2f(fmaf(s[a][i >> 2][i & 3u], f, up));
+                float z = __builtin_amdgcn_exp2f(fmaf(s[a][i >> 2][(i & 3u) + 1u], f, up));
                 if constexpr (edge) {{ p = at + i < see[a] ? p : 0.0f; z = at + i + 1u < see[a] ? z : 0.0f; }}
                 sum += p + z;
                 halves(p, z, minus, p1[a][i >> 3].p[(i & 7u) >> 1], p2[a][i >> 3].w[(i & 7u) >> 1]);

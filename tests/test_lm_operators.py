@@ -751,6 +751,40 @@ def test_cache_attention_beside_a_block_of_zero_keys(G, later, tiles, waves, spl
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("tiles,waves,splits", [(1, 4, 1), (2, 4, 1), (1, 8, 1), (1, 4, 2)])
+@pytest.mark.parametrize("size", [1e4, 1e6, 1e8, 1e10, 1e16])
+@pytest.mark.parametrize("T", [1, 70])
+def test_cache_attention_of_scores_beyond_whole_numbers(T, size, tiles, waves, splits, monkeypatch):
+    """Scores so large that neighbouring numbers of 32 bits lie far apart: one token takes all the weight, and nothing overflows."""
+    require_gpu()
+    monkeypatch.setattr(HIPLM, "attend_tiles", staticmethod(lambda *a: tiles))
+    monkeypatch.setattr(HIPLM, "attend_waves", staticmethod(lambda *a: waves))
+    monkeypatch.setattr(HIPLM, "attend_splits", staticmethod(lambda *a: splits))
+    rng = np.random.default_rng(41)
+    first, d = 600, 64
+    n = first + T
+    k, v = rows_of(rng, 1, n, d)
+    q = (rng.standard_normal((1, T, 4 * d)) * size).astype(f32)
+    cache = filled(1, n, 1, d, (k[:, :first], v[:, :first]))
+    cache.write(hip_tensor(k[:, first:]), hip_tensor(v[:, first:]))
+    y = cache.attend(hip_tensor(q), 0.125).numpy().reshape(T, 4, d)
+    assert np.isfinite(y).all()
+    kk, vv = (held(a[0].reshape(n, 1, d), n // 64 * 64)[:, 0] for a in (k, v))
+    alone = 0
+    for t in range(T):
+        for j in range(4):
+            s = kk[:first + t + 1].astype(np.float64) @ q[0, t, j * d:(j + 1) * d].astype(np.float64) * 0.125
+            # a score is off by (d + 4) roundings of the largest sum of |q k|; where the best one leads by more than 40 and that, it is alone
+            off = (np.abs(kk[:first + t + 1]) @ np.abs(q[0, t, j * d:(j + 1) * d])).max() * 0.125 * (d + 4) * EPS
+            two = np.partition(s, -2)[-2:]
+            if two[1] - two[0] > 40 + 4 * off:
+                alone += 1
+                # exp(-40) of 670 others is nothing; the weight and its reciprocal are off by 2^-21 and four roundings
+                within(y[t, j], vv[s.argmax()], np.abs(vv).max() * (2.0 ** -21 + 4 * EPS), f"row {t}, head {j}")
+    assert alone >= 3 * T
+
+
+@pytest.mark.gpu
 def test_cache_beyond_four_gigabytes():
     """Offsets past 32 bits: blocks that were never written have scale 0, so their tokens weigh exp(0) and add nothing."""
     require_gpu()

@@ -547,7 +547,7 @@ def cache8_attend_kernel(DP: int, NQ: int = 1, W: int = 4, stream: bool = False)
     A workgroup of W wavefronts per (NQ tiles of one key head, split of the blocks); they are joined through LDS in
     wavefront order.  With one split y is written; else O, m and l go to `part` and cache8_join_kernel adds the splits up
     in their order.  Bound by memory while few query rows share a key head, 2 bytes per token and column (16 sequences up to 32768
-    tokens, 32 heads on 8 of 128: 132 us, 6.2 TB/s); with many by issue, some 290 vector and 32 matrix instructions a block of 64 and
+    tokens, 32 heads on 8 of 128: 132 us, 6.2 TB/s); with many by issue, some 295 vector and 32 matrix instructions a block of 64 and
     tile of 16 rows, which do not overlap (4 x 12 heads of 64, 256 rows after 4096 tokens: 47 us, 285 TFLOP/s of the formula's
     operations); with few blocks by chains of dependent reads (one block and a tail: 3.9 us)."""
     ND, NK, Q4 = DP // 16, DP // 32, DP // 4             # column tiles of V^T, k steps of a score, columns a lane feeds

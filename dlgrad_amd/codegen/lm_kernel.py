@@ -269,6 +269,10 @@ static __device__ __forceinline__ void cache8_extent(const float* __restrict__ l
     n = c >= (float)T ? T : c > 0.0f ? (u32)c : 0u;
     n = min(n, cap - len);
 }
+// Whether a tail that says `mark` keeps the first `rows` (1 .. 63) rows of block blk: a mark is 64 * block + the rows that lie there.
+static __device__ __forceinline__ bool cache8_kept(u32 mark, u32 blk, u32 rows) {
+    return mark >= blk * 64u + rows && mark <= blk * 64u + 64u;
+}
 """
 
 
@@ -308,6 +312,11 @@ def cache8_write_kernel(DP: int, vec: bool) -> tuple[str, str, str]:
 
     A row that holds a NaN or an infinity is kept as NaN in the tail, and a block with such a row gets NaN for its scales:
     every output that sees it is NaN, and the codes stay whole numbers.
+
+    A call may be followed by one that starts at a smaller length than it ended at, or at its own again.  Both tails together hold what
+    that takes while the call touches two blocks; one that completes more leaves the rows of the blocks between nowhere in fp32, and
+    where it ends in the tail that it started in, those of its first block neither.  Each tail's mark says what lies there
+    (cache8_kept), and rows that are not there are NaN to whoever needs them.
 
     One workgroup of 512 threads per (block of 64, head, sequence), a thread per four columns of a row (DP / 32 times).  With 256 a
     launch of few workgroups, which is one pass over the code, takes longer (2 x 12 heads of 64, 512 tokens: 6.7 us against 5.4),
@@ -363,20 +372,23 @@ static __device__ __forceinline__ bool odd_one(float x) {{ return !(fabsf(x) < _
 static __device__ __forceinline__ bool odd4(float4 f) {{ return odd_one(f.x) || odd_one(f.y) || odd_one(f.z) || odd_one(f.w); }}
 extern "C" __global__ __launch_bounds__({NT}) void {name}(const float* __restrict__ k, const float* __restrict__ v,
         const float* __restrict__ lengths, const float* __restrict__ counts,
-        unsigned char* __restrict__ kc, unsigned char* __restrict__ vc, float* __restrict__ scales, float* tail_k, float* tail_v,
+        unsigned char* __restrict__ kc, unsigned char* __restrict__ vc, float* __restrict__ scales, float* tail_k, float* tail_v, u32* marks,
         u32 T, u32 H, u32 d, u32 NB, u32 kp, u32 vp) {{
     __shared__ __attribute__((aligned(16))) u32 kt[DP * 16u], vt[DP * 16u];       // the block's bytes
     __shared__ float sk[{NT // 64}], sv[{NT // 64}];
     __shared__ u32 bad[64];
     const u32 t = threadIdx.x, lane = t & 63u, h = blockIdx.y, b = blockIdx.z;
     u32 len, n;
-    cache8_extent(lengths, counts, b, T, NB * 64u, len, n);
-    if (!n) return;
-    const u32 total = len + n, first = len >> 6, last = total >> 6;         // last: the block that is not full afterwards
     const u64 bh = (u64)b * H + h, heads = (u64)gridDim.z * H;
+    const uint2 was = *reinterpret_cast<const uint2*>(marks + 2u * bh);       // (written by workgroup 0 alone, which alone goes by them)
+    cache8_extent(lengths, counts, b, T, NB * 64u, len, n);
+    const u32 total = len + n, first = len >> 6, last = total >> 6;         // last: the block that is not full afterwards
+    const u32 mine = first & 1u ? was.y : was.x, other = first & 1u ? was.x : was.y;
+    const bool lost = (len & 63u) && !cache8_kept(mine, first, len & 63u);      // the rows before this call are not in their tail
+    if (!n && blockIdx.x) return;
     const float* __restrict__ kh = k + (u64)b * T * kp + (u64)h * d;
     const float* __restrict__ vh = v + (u64)b * T * vp + (u64)h * d;
-    for (u32 pass = 0; pass < 2u; ++pass) {{
+    for (u32 pass = n ? 0u : 2u; pass < 2u; ++pass) {{
         const u32 blk = pass ? last : first + blockIdx.x;
         if (pass && (blockIdx.x != 0u || last == first || !(total & 63u))) break;       // (uniform over the workgroup)
         const bool full = blk < last;
@@ -421,7 +433,7 @@ extern "C" __global__ __launch_bounds__({NT}) void {name}(const float* __restric
             }}
         }}
         if (full) {{
-            const bool odd = __any(bad[lane] != 0u);
+            const bool odd = __any(bad[lane] != 0u) || (lost && blk == first);
             float ak = 0.0f, av = 0.0f;
             #pragma unroll
             for (u32 i = 0; i < {NT // 64}u; ++i) {{ ak = fmaxf(ak, sk[i]); av = fmaxf(av, sv[i]); }}
@@ -453,9 +465,20 @@ extern "C" __global__ __launch_bounds__({NT}) void {name}(const float* __restric
         }}
         __syncthreads();
     }}
+    if (blockIdx.x == 0u && t == 0u) {{                                     // (the passes' barriers lie after every thread's read of the marks)
+        const u32 f64 = first * 64u, l64 = last * 64u + (total & 63u);
+        // the first block's: what lay there, and the new rows where they were stored
+        u32 a = lost ? 0u : last == first ? l64 : last == first + 1u ? f64 + 64u : f64 + (len & 63u);
+        u32 o = other <= f64 ? other : 0u;                                  // the other one's: not what a call before this one put there in its place
+        if (last > first) {{
+            if ((last - first) & 1u) o = l64;
+            else if (total & 63u) a = l64;
+        }}
+        *reinterpret_cast<uint2*>(marks + 2u * bh) = first & 1u ? make_uint2(o, a) : make_uint2(a, o);
+    }}
 }}
 """
-    return src, name, _fmt("P" * 9, "I" * 6)
+    return src, name, _fmt("P" * 10, "I" * 6)
 
 
 @cache
@@ -467,7 +490,7 @@ def cache8_read_kernel(DP: int) -> tuple[str, str, str]:
     5.6 TB/s)."""
     name = f"cache8_read_d{DP}"
     src = f"""{PRELUDE}{_CACHE8}{_cache8_layout(DP)}extern "C" __global__ __launch_bounds__(256) void {name}(const unsigned char* __restrict__ kc, const unsigned char* __restrict__ vc,
-        const float* __restrict__ scales, const float* __restrict__ tail_k, const float* __restrict__ tail_v,
+        const float* __restrict__ scales, const float* __restrict__ tail_k, const float* __restrict__ tail_v, const u32* __restrict__ marks,
         const float* __restrict__ lengths, const float* __restrict__ counts, float* __restrict__ ko, float* __restrict__ vo,
         u32 N, u32 H, u32 d, u32 NB, u32 extra) {{
     __shared__ __attribute__((aligned(16))) u32 kt[DP * 16u], vt[DP * 16u];       // the block's bytes
@@ -488,6 +511,7 @@ def cache8_read_kernel(DP: int) -> tuple[str, str, str]:
     __syncthreads();
     const float* __restrict__ tk = tail_k + (((u64)(blk & 1u) * heads + bh) * 64u) * DP;
     const float* __restrict__ tv = tail_v + (((u64)(blk & 1u) * heads + bh) * 64u) * DP;
+    const bool lost = blk == last && (total & 63u) && !cache8_kept(marks[2u * bh + (blk & 1u)], blk, total & 63u);
     const u64 C = (u64)H * d;
     // four columns a thread (as many of them as there are)
     for (u32 i = t; i < 64u * {DP // 4}u; i += 256u) {{
@@ -503,6 +527,7 @@ def cache8_read_kernel(DP: int) -> tuple[str, str, str]:
         }} else if (p < total) {{
             x = *reinterpret_cast<const float4*>(tk + row * DP + c);
             z = *reinterpret_cast<const float4*>(tv + row * DP + c);
+            if (lost) {{ const float no = __builtin_nanf(""); x = make_float4(no, no, no, no); z = x; }}
         }}
         const u64 o = ((u64)b * N + p) * C + (u64)h * d + c;
         if ((d & 3u) == 0u) {{                                              // (fresh results are aligned)
@@ -517,7 +542,7 @@ def cache8_read_kernel(DP: int) -> tuple[str, str, str]:
     }}
 }}
 """
-    return src, name, _fmt("P" * 9, "I" * 5)
+    return src, name, _fmt("P" * 10, "I" * 5)
 
 
 @cache
@@ -604,7 +629,7 @@ struct Inside {{ static constexpr bool edge = false; }};
 struct Edge {{ static constexpr bool edge = true; }};
 extern "C" __global__ __launch_bounds__({bounds}) void {name}(const float* __restrict__ q, const unsigned char* __restrict__ kc,
         const unsigned char* __restrict__ vc, const float* __restrict__ scales, const float* __restrict__ tail_k, const float* __restrict__ tail_v,
-        const float* __restrict__ lengths, const float* __restrict__ counts, float* __restrict__ y, float* __restrict__ part,
+        const u32* __restrict__ marks, const float* __restrict__ lengths, const float* __restrict__ counts, float* __restrict__ y, float* __restrict__ part,
         u32 B, u32 T, u32 H, u32 group, u32 d, u32 NB, u32 tiles, u32 splits, u32 q_wide, float scale) {{
     __shared__ float so[W][16][DP + 4u];
     __shared__ float sm[W][16], sl[W][16];
@@ -784,6 +809,7 @@ extern "C" __global__ __launch_bounds__({bounds}) void {name}(const float* __res
         const float* __restrict__ tk = tail_k + (((u64)(last & 1u) * heads + bh) * 64u + 16u * tt) * DP;
         const float* __restrict__ tv = tail_v + (((u64)(last & 1u) * heads + bh) * 64u + 16u * tt) * DP;
         const u32 p0 = last * 64u + 16u * tt + 4u * g;                              // this lane's four tokens
+        const u32 mark = marks[2u * bh + (last & 1u)];
         float kt[{Q4}], vt[ND][4];                                                  // (both on their way before the first is used)
         #pragma unroll
         for (u32 i = 0; i < {Q4}u; ++i) kt[i] = tk[r * DP + g * {Q4}u + i];
@@ -791,15 +817,17 @@ extern "C" __global__ __launch_bounds__({bounds}) void {name}(const float* __res
         for (u32 dt = 0; dt < ND; ++dt)
             #pragma unroll
             for (u32 i = 0; i < 4u; ++i) vt[dt][i] = tv[(4u * g + i) * DP + dt * 16u + r];
+        const bool kept = cache8_kept(mark, last, (len + n) & 63u);                     // (else: NaN to every query that sees some of it)
         #pragma unroll
         for (u32 a = 0; a < NQ; ++a) {{
+            const float turn = kept ? back[a] : __builtin_nanf("");
             f4 acc = (f4){{0.f, 0.f, 0.f, 0.f}};
             #pragma unroll
             for (u32 i = 0; i < {Q4}u; ++i) acc = MFMA32(kt[i], (float)q1[a][i >> 3].e[i & 7u] + (float)q2[a][i >> 3].e[i & 7u], acc);
             float mx = NINF;
             #pragma unroll
             for (u32 i = 0; i < 4u; ++i) {{
-                acc[i] = p0 + i < see[a] ? acc[i] * back[a] : NINF;
+                acc[i] = p0 + i < see[a] ? acc[i] * turn : NINF;
                 mx = fmaxf(mx, acc[i]);
             }}
             mx = four_max(mx);
@@ -852,7 +880,7 @@ extern "C" __global__ __launch_bounds__({bounds}) void {name}(const float* __res
     }}
 }}
 """
-    return src, name, _fmt("P" * 10, "I" * 9, "f")
+    return src, name, _fmt("P" * 11, "I" * 9, "f")
 
 
 CACHE8_MAX_SPLITS = 64      # what one wavefront joins: a lane per split

@@ -228,8 +228,10 @@ class QuantizedKVCache:
     any length.  counts (B, 1): how many of the T rows of each sequence are tokens (a padded batch); the rest is neither
     written nor seen, and their rows of the result are zeros.  Rows that do not fit into the capacity (rounded up to whole blocks) are
     dropped the same way.  Until advance(), a write of at most 64 rows may be repeated or replaced, and advance() may be given
-    less than was written; a longer one can be repeated where every sequence holds whole blocks.  A row with a NaN or an
-    infinity makes every result that sees its block, once that is full, or itself, before, NaN.  Values are to stay below 2^88 in
+    less than was written.  After a longer one a sequence goes on from all that was written or from a whole block of it, and it can be
+    repeated where the sequence holds whole blocks: the tokens of any other block that is opened again are gone, and every result
+    that sees it is NaN (a batch of padded prompts therefore gives write() its counts).  A row with a NaN or an infinity makes
+    every result that sees its block, once that is full, or itself, before, NaN.  Values are to stay below 2^88 in
     magnitude.  Results carry no tape.
 
     Query heads share key heads in order: query heads h * G .. h * G + G - 1 read key head h, G = n_head / n_kv_head."""

@@ -29,8 +29,8 @@ def _on_device(what: str, **tensors) -> None:
 
 
 class Cache8:
-    """One layer of an 8-bit key/value cache in device memory: codes, scales and the fp32 tails."""
-    __slots__ = ("batch", "heads", "d", "width", "blocks", "layers", "kc", "vc", "scales", "tail_k", "tail_v", "writers", "attenders")
+    """One layer of an 8-bit key/value cache in device memory: codes, scales, the fp32 tails and what each tail holds."""
+    __slots__ = ("batch", "heads", "d", "width", "blocks", "layers", "kc", "vc", "scales", "tail_k", "tail_v", "marks", "writers", "attenders")
 
     def __init__(self, batch: int, heads: int, d: int, blocks: int, layers: int = 1) -> None:
         """layers: how many of these a step reads one after the other."""
@@ -43,9 +43,11 @@ class Cache8:
         self.scales = Buffer.full((n, 2), 0.0, Device.HIP)
         # tails are read in whole blocks: columns beyond d, and rows not written yet, are zeros from the start
         self.tail_k, self.tail_v = (Buffer.full((2, batch * heads, K.CACHE8_BLOCK, self.width), 0.0, Device.HIP) for _ in range(2))
+        self.marks = Buffer.full((batch * heads, 2), 0.0, Device.HIP)         # (whole numbers of 32 bits, 0: nothing)
 
     @property
     def nbytes(self) -> int:
+        """Bytes of codes, scales and tails (the marks are 8 more for each sequence and head)."""
         return self.kc.nbytes + self.vc.nbytes + self.scales.nbytes + self.tail_k.nbytes + self.tail_v.nbytes
 
 
@@ -157,8 +159,10 @@ class HIPLM:
         T = shape[1]
         if T > c.blocks * K.CACHE8_BLOCK:
             raise ValueError(f"cache8_write: {T} tokens for a cache of {c.blocks * K.CACHE8_BLOCK}")
+        if not T:
+            return lambda ka, va, la, ca: None
         grid, wide, kernels = (-(-T // K.CACHE8_BLOCK), c.heads, c.batch), C % 4 == 0 and c.d % 4 == 0, [None, None]
-        tail = (c.kc.addr, c.vc.addr, _addr(c.scales), _addr(c.tail_k), _addr(c.tail_v), T, c.heads, c.d, c.blocks, C, C)
+        tail = (c.kc.addr, c.vc.addr, _addr(c.scales), _addr(c.tail_k), _addr(c.tail_v), _addr(c.marks), T, c.heads, c.d, c.blocks, C, C)
 
         def run(ka: int, va: int, la: int, ca: int) -> None:
             vec = wide and not (ka | va) & 15
@@ -167,7 +171,7 @@ class HIPLM:
                 k = kernels[vec] = kernel(K.cache8_write_kernel, c.width, vec)
             # a call completes at most ceil(T / 64) blocks, the one it starts in among them
             launch(k, grid, K.CACHE8_WRITE_THREADS, ka, va, la, ca, *tail)
-        return run if T else lambda ka, va, la, ca: None
+        return run
 
     @staticmethod
     @dispatcher.register(CustomOps.CACHE8_WRITE, Device.HIP)
@@ -235,7 +239,7 @@ class HIPLM:
         if grid >= 2 ** 31 or pairs * rows >= 2 ** 31:
             raise ValueError(f"cache8_attend: {pairs} heads of {rows} query rows exceed the grid")
         k, join = kernel(K.cache8_attend_kernel, c.width, nq, waves, HIPLM.attend_streams(c, tiles)), kernel(K.cache8_join_kernel, c.width) if splits > 1 else None
-        held = (c.kc.addr, c.vc.addr, _addr(c.scales), _addr(c.tail_k), _addr(c.tail_v))
+        held = (c.kc.addr, c.vc.addr, _addr(c.scales), _addr(c.tail_k), _addr(c.tail_v), _addr(c.marks))
         sizes = (c.batch, T, c.heads, group, c.d, c.blocks, tiles, splits)
         wide = c.d % 4 == 0                                              # (then the rows of the queries are whole 16-byte items)
         n_part, join_grid, join_sizes = pairs * rows * splits * (c.width + 2), (pairs * rows + 3) // 4, (pairs * rows, T, c.heads, group, c.d, splits)
@@ -272,7 +276,7 @@ class HIPLM:
         k, v = alloc(size), alloc(size)
         if size:
             launch(kernel(K.cache8_read_kernel, c.width), (-(-n // K.CACHE8_BLOCK), c.heads, c.batch), 256, c.kc.addr, c.vc.addr, _addr(c.scales),
-                   _addr(c.tail_k), _addr(c.tail_v), _addr(lengths), _addr(counts) if counts is not None else 0, k.addr, v.addr,
+                   _addr(c.tail_k), _addr(c.tail_v), _addr(c.marks), _addr(lengths), _addr(counts) if counts is not None else 0, k.addr, v.addr,
                    n, c.heads, c.d, c.blocks, extra)
         return k, v
 

@@ -704,6 +704,94 @@ def test_cache_goes_back_over_rows_that_were_not_kept():
 
 
 @pytest.mark.gpu
+def test_cache_goes_on_from_less_than_a_long_write():
+    """Rows that a long write did not leave in fp32 are NaN where they are needed, and not the rows of other tokens."""
+    require_gpu()
+    rng = np.random.default_rng(40)
+    k, v = rows_of(rng, 1, 200, 32)
+    q = rng.standard_normal((1, 1, 32)).astype(f32)
+    one = lambda: [hip_tensor(a) for a in rows_of(rng, 1, 1, 32)]                                   # noqa: E731
+
+    def check(cache, n, right, what):
+        got = [t.numpy()[0] for t in cache.read(n)]
+        cache.write(*one())
+        y = cache.attend(hip_tensor(q)).numpy()
+        if hip.COMPILE_ONLY:
+            return
+        for a, src in zip(got, (k, v)):
+            want = held(src[0, :n].reshape(n, 1, 32), n // 64 * 64).reshape(n, 32)
+            same(a[:n // 64 * 64], want[:n // 64 * 64], what)
+            if right:
+                same(a, want, what)
+            else:
+                assert np.isnan(a[n // 64 * 64:]).all(), what
+        assert np.isfinite(y).all() if right else np.isnan(y).all(), what
+
+    for tried, n, right in ((200, 70, False), (200, 128, True), (200, 192, True), (200, 195, True), (130, 100, False), (130, 10, False), (128, 64, True), (100, 70, True), (100, 3, True)):
+        cache = nn.QuantizedKVCache(1, 256, 1, 32)
+        cache.write(hip_tensor(k[:, :tried]), hip_tensor(v[:, :tried]))
+        cache.advance(n)
+        check(cache, n, right, f"{tried} tried, {n} kept")
+    cache = filled(1, 256, 1, 32, (k[:, :10], v[:, :10]))
+    for time, right in (("once", True), ("twice", False)):                      # the second time the ten rows before it are gone
+        cache.write(hip_tensor(k[:, 10:140]), hip_tensor(v[:, 10:140]))
+        got = cache.read(140, new=130)[0].numpy()[0]
+        if not hip.COMPILE_ONLY:
+            same(got[64:], held(k[0, :140].reshape(140, 1, 32), 128).reshape(140, 32)[64:], time)
+            assert np.isfinite(got[:64]).all() if right else np.isnan(got[:64]).all(), time
+    cache = filled(1, 256, 1, 32, (k[:, :10], v[:, :10]))
+    cache.write(hip_tensor(k[:, 50:70]), hip_tensor(v[:, 50:70]))                # tried, and given up for a longer one
+    cache.write(hip_tensor(k[:, 10:200]), hip_tensor(v[:, 10:200]))
+    cache.advance(15)
+    got = cache.read(25)[0].numpy()[0]
+    if not hip.COMPILE_ONLY:
+        assert np.isnan(got).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("seed", range(6))
+def test_cache_gives_its_own_tokens_or_nan(seed):
+    """Writes of any length, replaced and advanced over by any part of them: every position reads as its token, or as NaN in a block that
+    the documentation says is gone."""
+    require_gpu()
+    if hip.COMPILE_ONLY:
+        return
+    rng = np.random.default_rng(seed)
+    B, H, d, cap = 3, 2, 32, 1024
+    C, at, gone = H * d, np.zeros(B, int), [set() for _ in range(B)]
+    truth = np.zeros((2, B, cap, C), f32)
+    cache = nn.QuantizedKVCache(B, cap, H, d)
+    while at.max() < cap - 320:
+        for again in range(rng.integers(1, 3)):
+            T = int(rng.choice([1, 7, 64, 65, 130, 200, 300]))
+            n = np.where(rng.random(B) < 0.5, T, rng.integers(0, T + 1, B))
+            new = rows_of(rng, B, T, C)
+            if again:
+                for b in range(B):
+                    if at[b] % 64 and before[b] > 64:
+                        gone[b].add(at[b] // 64)
+            cache.write(hip_tensor(new[0]), hip_tensor(new[1]), counts=hip_tensor(n.reshape(B, 1)))
+            before = n
+            for b in range(B):
+                truth[:, b, at[b]:at[b] + n[b]] = [a[b, :n[b]] for a in new]
+        m = np.where(rng.random(B) < 0.5, n, rng.integers(0, n + 1))
+        for b in range(B):
+            if n[b] > 64 and m[b] < n[b] and (at[b] + m[b]) % 64 and (at[b] + m[b]) // 64 != (at[b] + n[b]) // 64:
+                gone[b].add((at[b] + m[b]) // 64)
+        cache.advance(hip_tensor(m.reshape(B, 1)))
+        at += m
+        for name, a, src in zip("kv", cache.read(cap), truth):
+            a = a.numpy()
+            for b in range(B):
+                want = held(src[b, :at[b]].reshape(-1, H, d), at[b] // 64 * 64).reshape(-1, C)
+                for blk in range(-(-at[b] // 64)):
+                    rows = slice(blk * 64, min(blk * 64 + 64, at[b]))
+                    if not (blk in gone[b] and np.isnan(a[b, rows]).any()):
+                        same(a[b, rows], want[rows], f"{name} of sequence {b}, block {blk}")
+                assert (a[b, at[b]:] == 0).all()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("gap", [14, 24, 30, 36])
 def test_cache_attention_adds_up_many_small_weights(gap):
     """2^20 tokens of weight 2^-gap beside one of weight 1, values around 1: together they move the result by up to 2^(20 - gap)."""

@@ -373,7 +373,7 @@ static __device__ __forceinline__ bool odd4(float4 f) {{ return odd_one(f.x) || 
 extern "C" __global__ __launch_bounds__({NT}) void {name}(const float* __restrict__ k, const float* __restrict__ v,
         const float* __restrict__ lengths, const float* __restrict__ counts,
         unsigned char* __restrict__ kc, unsigned char* __restrict__ vc, float* __restrict__ scales, float* tail_k, float* tail_v, u32* marks,
-        u32 T, u32 H, u32 d, u32 NB, u32 kp, u32 vp) {{
+        u32* __restrict__ wrote, u32 T, u32 H, u32 d, u32 NB, u32 kp, u32 vp) {{
     __shared__ __attribute__((aligned(16))) u32 kt[DP * 16u], vt[DP * 16u];       // the block's bytes
     __shared__ float sk[{NT // 64}], sv[{NT // 64}];
     __shared__ u32 bad[64];
@@ -465,6 +465,7 @@ extern "C" __global__ __launch_bounds__({NT}) void {name}(const float* __restric
         }}
         __syncthreads();
     }}
+    if (blockIdx.x == 0u && h == 0u && t == 0u) wrote[b] = n;
     if (blockIdx.x == 0u && t == 0u) {{                                     // (the passes' barriers lie after every thread's read of the marks)
         const u32 f64 = first * 64u, l64 = last * 64u + (total & 63u);
         // the first block's: what lay there, and the new rows where they were stored
@@ -478,7 +479,26 @@ extern "C" __global__ __launch_bounds__({NT}) void {name}(const float* __restric
     }}
 }}
 """
-    return src, name, _fmt("P" * 10, "I" * 6)
+    return src, name, _fmt("P" * 11, "I" * 6)
+
+
+@cache
+def cache8_advance_kernel() -> tuple[str, str, str]:
+    """lengths[b] += by[b], or `all` for every sequence, as the whole number of rows it stands for and no more than the last write
+    brought and an earlier advance left of them (wrote[b]); reset: everything to 0.  A launch and nothing else: three numbers a sequence."""
+    src = f"""{PRELUDE}{_CACHE8}
+extern "C" __global__ __launch_bounds__(256) void cache8_advance(float* __restrict__ lengths, const float* __restrict__ by, u32* __restrict__ wrote,
+        u32 B, u32 cap, u32 all, u32 reset) {{
+    const u32 b = blockIdx.x * 256u + threadIdx.x;
+    if (b >= B) return;
+    u32 len, n;
+    const u32 w = wrote[b];
+    cache8_extent(lengths, by, b, by ? w : min(w, all), cap, len, n);
+    lengths[b] = reset ? 0.0f : (float)(len + n);
+    wrote[b] = reset ? 0u : w - n;
+}}
+"""
+    return src, "cache8_advance", _fmt("P" * 3, "I" * 4)
 
 
 @cache

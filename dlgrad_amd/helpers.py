@@ -104,6 +104,7 @@ class CustomOps(_Op):
     CACHE8_WRITE = auto()           # new keys and values into the 8-bit cache: blocks of 64 tokens and a head quantised as they fill up
     CACHE8_ATTEND = auto()          # attention of new positions over the 8-bit cache
     CACHE8_READ = auto()            # the values that the 8-bit cache stands for
+    CACHE8_ADVANCE = auto()         # its lengths after what has been written
     ADJUST_LOGITS = auto()          # penalties for tokens said before, a bias and a mask on logits, one kernel
     RMSNORM = auto()                # (x * rsqrt(mean(x^2) + eps)) * w over the last axis, one kernel
     RMSNORM_BWD = auto()            # its backward: dx in one kernel, dw by partial rows + a column sum

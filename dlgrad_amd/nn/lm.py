@@ -254,7 +254,9 @@ class QuantizedKVCache:
         blocks = -(-capacity // self.BLOCK)
         self.capacity = blocks * self.BLOCK
         self.lengths = Tensor.full((batch, 1), 0.0, device="hip") if lengths is None else lengths
-        self.layers = [Cache8(batch, n_kv_head, head_dim, blocks, layers) for _ in range(layers)]
+        wrote = Buffer.full((batch, 1), 0.0, Device.HIP)                        # (whole numbers of 32 bits)
+        self.layers = [Cache8(batch, n_kv_head, head_dim, blocks, layers, wrote) for _ in range(layers)]
+        self._most = 0                                                          # rows of the longest write so far
 
     @property
     def nbytes(self) -> int:
@@ -286,6 +288,7 @@ class QuantizedKVCache:
             run(kd.ptr.addr, vd.ptr.addr, self.lengths.data.ptr.addr, 0 if counts is None else counts.data.ptr.addr)
         else:
             self._run(CustomOps.CACHE8_WRITE, layer, counts, k=kd, v=vd)
+            self._most = max(self._most, kd.shape[1])
 
     def attend(self, q: Tensor, scale: float | None = None, layer: int = 0, counts: Tensor | None = None) -> Tensor:
         """q (B, T, n_head * head_dim): the queries of positions lengths[b] .., whose keys and values write() has stored; each sees
@@ -309,20 +312,25 @@ class QuantizedKVCache:
         return _result(Buffer.fresh(k, shape, Device.HIP)), _result(Buffer.fresh(v, shape, Device.HIP))
 
     def advance(self, n: "int | Tensor") -> None:
-        """The rows written become part of the sequences: n of each, or n (B, 1) of them."""
+        """The rows written become part of the sequences: n of each, or n (B, 1) of them, taken as write() takes its counts.  A sequence goes on
+        by no more rows than the last write brought it, and never back."""
         if isinstance(n, Tensor):
             if n.numel != self.batch or n.device is not Device.HIP or n.data.is_host_scalar:
                 raise ValueError(f"advance: counts {n.shape} for {self.batch} sequences")
-            step = Tensor(n.data.reshape(self.lengths.shape))
-        elif n < 0 or n != int(n):
-            raise ValueError(f"advance: {n} tokens (a cache does not go back; see reset())")
+            by = n.data
+        elif not 0 <= n <= self._most or n != int(n):
+            raise ValueError(f"advance: {n} tokens after writes of at most {self._most} (a cache does not go back; see reset())")
         else:
-            step = float(n)
-        self.lengths.data.copy_((self.lengths + step).clamp(max=self.capacity).data)
+            by = int(n)
+        self._move(by)
 
     def reset(self) -> None:
         """Forgets every token."""
-        self.lengths.data.copy_(Tensor.full(self.lengths.shape, 0.0, device="hip").data)
+        self._move(0, reset=True)
+
+    def _move(self, by: "Buffer | int", reset: bool = False) -> None:
+        self.lengths.data._writable("advance")
+        _dispatch_table[(CustomOps.CACHE8_ADVANCE, Device.HIP)](cache=self.layers[0], lengths=self.lengths.data, by=by, reset=reset)
 
 
 _adjust_plans: dict = {}       # shapes and numbers that _check_adjust has let through -> the launch

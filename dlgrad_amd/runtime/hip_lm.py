@@ -30,10 +30,11 @@ def _on_device(what: str, **tensors) -> None:
 
 class Cache8:
     """One layer of an 8-bit key/value cache in device memory: codes, scales, the fp32 tails and what each tail holds."""
-    __slots__ = ("batch", "heads", "d", "width", "blocks", "layers", "kc", "vc", "scales", "tail_k", "tail_v", "marks", "writers", "attenders")
+    __slots__ = ("batch", "heads", "d", "width", "blocks", "layers", "kc", "vc", "scales", "tail_k", "tail_v", "marks", "wrote", "writers", "attenders")
 
-    def __init__(self, batch: int, heads: int, d: int, blocks: int, layers: int = 1) -> None:
-        """layers: how many of these a step reads one after the other."""
+    def __init__(self, batch: int, heads: int, d: int, blocks: int, layers: int, wrote: Buffer) -> None:
+        """layers: how many of these a step reads one after the other.  wrote: rows of each sequence that the last write to any of them brought."""
+        self.wrote = wrote
         self.batch, self.heads, self.d, self.blocks, self.layers = batch, heads, d, blocks, layers
         self.width = K.cache8_width(d)
         self.writers, self.attenders = _PlanCache(), _PlanCache()            # shape of a call -> the launch that its checks ended in
@@ -162,7 +163,7 @@ class HIPLM:
         if not T:
             return lambda ka, va, la, ca: None
         grid, wide, kernels = (-(-T // K.CACHE8_BLOCK), c.heads, c.batch), C % 4 == 0 and c.d % 4 == 0, [None, None]
-        tail = (c.kc.addr, c.vc.addr, _addr(c.scales), _addr(c.tail_k), _addr(c.tail_v), _addr(c.marks), T, c.heads, c.d, c.blocks, C, C)
+        tail = (c.kc.addr, c.vc.addr, _addr(c.scales), _addr(c.tail_k), _addr(c.tail_v), _addr(c.marks), _addr(c.wrote), T, c.heads, c.d, c.blocks, C, C)
 
         def run(ka: int, va: int, la: int, ca: int) -> None:
             vec = wide and not (ka | va) & 15
@@ -279,6 +280,17 @@ class HIPLM:
                    _addr(c.tail_k), _addr(c.tail_v), _addr(c.marks), _addr(lengths), _addr(counts) if counts is not None else 0, k.addr, v.addr,
                    n, c.heads, c.d, c.blocks, extra)
         return k, v
+
+    @staticmethod
+    @dispatcher.register(CustomOps.CACHE8_ADVANCE, Device.HIP)
+    def cache8_advance(cache: Cache8, lengths: Buffer, by: "Buffer | int", reset: bool = False) -> None:
+        """by: rows of every sequence, or a number for each."""
+        counts = by if isinstance(by, Buffer) else None
+        HIPLM._cache8_lengths("cache8_advance", cache, lengths, counts)
+        if counts is None and not 0 <= by < 2 ** 32:
+            raise ValueError(f"cache8_advance: {by} rows")
+        launch(kernel(K.cache8_advance_kernel), -(-cache.batch // 256), 256, _addr(lengths), 0 if counts is None else _addr(counts), _addr(cache.wrote),
+               cache.batch, cache.blocks * K.CACHE8_BLOCK, by if counts is None else 0, int(reset))
 
     # ---- logits ----------------------------------------------------------------------------------------
     @staticmethod

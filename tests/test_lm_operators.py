@@ -749,6 +749,58 @@ def test_cache_goes_on_from_less_than_a_long_write():
 
 
 @pytest.mark.gpu
+def test_cache_advances_over_what_was_written():
+    """Counts below zero, beyond the rows of the write, between two whole numbers and without a value are what write() takes them for."""
+    require_gpu()
+    rng = np.random.default_rng(43)
+    B = 6
+    k, v = rows_of(rng, B, 5, 32)
+    c = np.array([[-3], [2.75], [9], [np.nan], [5], [0]], f32)
+    for brought in (True, False):
+        cache = nn.QuantizedKVCache(B, 128, 1, 32)
+        cache.write(hip_tensor(k), hip_tensor(v))
+        cache.advance(1)
+        cache.write(hip_tensor(k), hip_tensor(v), counts=hip_tensor(c) if brought else None)
+        cache.advance(hip_tensor(c))
+        same(cache.lengths.numpy().reshape(-1), [1, 3, 6, 1, 6, 1])
+        cache.advance(hip_tensor(np.full((B, 1), -1.0)))
+        same(cache.lengths.numpy().reshape(-1), [1, 3, 6, 1, 6, 1], "never back")
+        cache.advance(4)                                                      # what the write brought and was not taken yet
+        same(cache.lengths.numpy().reshape(-1), [1, 3, 6, 1, 6, 1] if brought else [5, 6, 6, 5, 6, 5])
+        got = cache.read(8)[0].numpy()
+        if not hip.COMPILE_ONLY:
+            for b, n in enumerate([1, 3, 6, 1, 6, 1] if brought else [5, 6, 6, 5, 6, 5]):
+                same(got[b, :n], np.concatenate([k[b, :1], k[b]])[:n])
+                assert (got[b, n:] == 0).all()
+    whole = nn.QuantizedKVCache(1, 64, 1, 32, lengths=hip_tensor([[7.0]]))
+    with pytest.raises(ValueError):
+        whole.advance(1)                                                       # nothing was ever written
+    whole.write(hip_tensor(k[:1, :2]), hip_tensor(v[:1, :2]))
+    for bad in (3, float("inf"), float("nan"), -1, 0.5):
+        with pytest.raises(ValueError):
+            whole.advance(bad)
+    whole.advance(1)
+    same(whole.lengths.numpy(), [[8.0]])
+    whole.reset()
+    whole.advance(2)
+    same(whole.lengths.numpy(), [[0.0]], "a reset forgets what was written")
+
+
+def test_cache_runtime_refuses_to_advance_by_what_does_not_fit():
+    """Host checks, before any device is touched."""
+    from dlgrad_amd.runtime.hip_lm import Cache8
+
+    class Ptr:
+        addr, nbytes = 256, 1 << 40
+    b = lambda *s: Buffer(Ptr(), s, Device.HIP)                  # noqa: E731
+    c = Cache8.__new__(Cache8)
+    c.batch, c.blocks, c.wrote = 2, 2, b(2, 1)
+    for lengths, by in ((b(2), b(3)), (b(3), 1), (b(2), -1), (b(2), 2 ** 32), (b(2), Buffer.from_scalar(1.0)), (Buffer.from_scalar(1.0), 1)):
+        with pytest.raises(ValueError):
+            HIPLM.cache8_advance(c, lengths, by)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("seed", range(6))
 def test_cache_gives_its_own_tokens_or_nan(seed):
     """Writes of any length, replaced and advanced over by any part of them: every position reads as its token, or as NaN in a block that

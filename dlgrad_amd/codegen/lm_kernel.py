@@ -572,11 +572,13 @@ def cache8_attend_kernel(DP: int, NQ: int = 1, W: int = 4, stream: bool = False)
     own; `group` query heads share a key head.  q and y are (B, T, H * group * d).  A row beyond counts[b] gives zeros.
 
     The codes are whole numbers of at most 127 and therefore exact in 16-bit floats, so the matrix units do the work:
-    a query row is scaled by a power of two to at most 2^15 and cut into two 16-bit floats, q' = q1 + q2 (22 bits and more of
-    it), and S^T = K (q1 + q2)^T has fp32 accuracy from two v_mfma_f32_16x16x32_f16 per 32 columns.  The probabilities go the
-    same way: p' = 2^15 exp(s - m) = p1 + p2 (p1 rounded to nearest, the rest, of either sign, cut off after 11 bits: 2^-22 of p'),
-    and the factor cancels in p' V / sum p'.  The scales enter in 32 bits, the keys' with the scores, the values' as a block's
-    product joins the running sum.
+    a query row is scaled by a power of two to at most 2^15 and held as two 16-bit floats an element, q' = q1 + q2 / 2^11: q1 the
+    nearest to q', q2 the nearest to what is left, 2^11 times.  That is q' to 2^-22 of itself or, where q2 runs into the smallest
+    steps of a 16-bit float, to 2^-36: 2^-50 of the row's largest element.  (Without the 2^11 they would begin at 2^-17 of the
+    largest, not 2^-28.)  S^T = K q1^T + K q2^T / 2^11 is two v_mfma_f32_16x16x32_f16 per 32 columns, added in 32 bits.  The probabilities go
+    the same way: p' = 2^15 exp(s - m) = p1 + p2 / 2^11, to 2^-22 of itself or 2^-51 of the largest one, which makes less than 2^-26 of it in the sum of
+    2^24 tokens; the factor 2^15 cancels in p' V / sum p'.  The scales enter in 32 bits, the keys' with the scores, the values' as a
+    block's product joins the running sum.
 
     A wavefront takes one block of 64 tokens at a time, for NQ tiles of 16 query rows, with (m, l, O) of its own.  Its lane
     r + 16 g (r < 16, g < 4) holds query r of each tile and, of every product S^T, four tokens; the rows of K are fed in the order
@@ -587,7 +589,7 @@ def cache8_attend_kernel(DP: int, NQ: int = 1, W: int = 4, stream: bool = False)
     one have been used, while its softmax runs, and its values likewise during the next scores.  stream: loads that leave no
     trace in the caches, for codes that are read once and would only displace others.
 
-    The tail, fp32, is shared out 16 tokens to a wavefront and goes through v_mfma_f32_16x16x4_f32, with q1 + q2 as the query.
+    The tail, fp32, is shared out 16 tokens to a wavefront and goes through v_mfma_f32_16x16x4_f32, with q1 + q2 / 2^11 as the query.
 
     A workgroup of W wavefronts per (NQ tiles of one key head, split of the blocks); they are joined through LDS in
     wavefront order.  With one split y is written; else O, m and l go to `part` and cache8_join_kernel adds the splits up
@@ -603,8 +605,39 @@ def cache8_attend_kernel(DP: int, NQ: int = 1, W: int = 4, stream: bool = False)
     fetch_k = fetch.format(f"reinterpret_cast<const u{kn}*>(p + u * {64 * Q4}u + i * {256 * kn}u)")
     fetch_v = fetch.format("reinterpret_cast<const u4*>(p + dt * 1024u)")
     half = ("i & 1u ? kr[u][i >> 1].z : kr[u][i >> 1].x, i & 1u ? kr[u][i >> 1].w : kr[u][i >> 1].y" if wide else "kr[u][i].x, kr[u][i].y")
-    # "256, 2" holds the kernel to 256 registers, with which the matrix instructions write ordinary ones; wider heads need more
-    bounds = "256, 2" if W == 4 and DP * NQ <= 128 else f"{64 * W}"
+    # "256, 2" holds the kernel to 256 registers, with which the matrix instructions write ordinary ones; wider heads need more.  "512, 4": 128, so that
+    # two workgroups of eight share a compute unit (48 x 12 heads of 64 over 600 tokens: 16.6 us against 20.4 with 158 registers); that takes the low
+    # products of the scores in the same accumulators, ahead of the high ones, where they have accumulators of their own otherwise (4 x 12
+    # heads of 64, 512 rows after 4096: 75.8 us, 80.1 in the same)
+    tight = W == 8 and NQ == 1 and DP <= 64
+    bounds = "256, 2" if W == 4 and DP * NQ <= 128 else "512, 4" if tight else f"{64 * W}"
+    if tight:
+        scores = f"""h8 k8[NK];
+            #pragma unroll
+            for (u32 i = 0; i < NK; ++i) k8[i] = widen({half});
+            s[0][u] = (f4){{0.f, 0.f, 0.f, 0.f}};
+            #pragma unroll
+            for (u32 i = 0; i < NK; ++i) s[0][u] = MFMA16(k8[i], q2[0][i].v, s[0][u]);
+            s[0][u] *= LOW;
+            #pragma unroll
+            for (u32 i = 0; i < NK; ++i) s[0][u] = MFMA16(k8[i], q1[0][i].v, s[0][u]);"""
+    else:
+        scores = f"""f4 low[NQ];
+            #pragma unroll
+            for (u32 a = 0; a < NQ; ++a) s[a][u] = low[a] = (f4){{0.f, 0.f, 0.f, 0.f}};
+            #pragma unroll
+            for (u32 i = 0; i < NK; ++i) {{
+                const h8 k8 = widen({half});
+                #pragma unroll
+                for (u32 a = 0; a < NQ; ++a) {{
+                    low[a] = MFMA16(k8, q2[a][i].v, low[a]);
+                    s[a][u] = MFMA16(k8, q1[a][i].v, s[a][u]);
+                }}
+            }}
+            #pragma unroll
+            for (u32 a = 0; a < NQ; ++a)
+                #pragma unroll
+                for (u32 i = 0; i < 4u; ++i) s[a][u][i] = fmaf(low[a][i], LOW, s[a][u][i]);"""
     src = f"""{PRELUDE}{_CACHE8}{_cache8_layout(DP)}#define ND {ND}u
 #define NK {NK}u
 #define NQ {NQ}u
@@ -619,6 +652,7 @@ union H8 {{ h8 v; h2 p[4]; _Float16 e[8]; u32 w[4]; }};
 #define MFMA16(a, b, c) __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0)
 #define MFMA32(a, b, c) __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0)
 #define NINF (-__builtin_inff())
+#define LOW 4.8828125e-4f                                                        // 2^-11
 // eight codes as 16-bit floats
 static __device__ __forceinline__ h8 widen(u32 lo, u32 hi) {{
     H8 r;
@@ -631,12 +665,13 @@ static __device__ __forceinline__ h8 widen(u32 lo, u32 hi) {{
     for (int i = 0; i < 4; ++i) r.p[i] += off;
     return r.v;
 }}
-// two numbers as the sum of two pairs of 16-bit floats; minus is -1 where the compiler does not see it: the subtraction
-// then takes the 16-bit float as it is, in one mixed multiply-add
-static __device__ __forceinline__ void halves(float a, float b, float minus, h2& hi, u32& lo) {{
+// two numbers as hi + lo / 2^11 in 16-bit floats.  minus is -1 where the compiler does not see it: the subtraction, which is exact, then
+// takes the 16-bit float as it is, in one mixed multiply-add
+static __device__ __forceinline__ void halves(float a, float b, float minus, h2& hi, h2& lo) {{
     const f2 x = {{a, b}};
     hi = __builtin_convertvector(x, h2);
-    lo = __builtin_bit_cast(u32, __builtin_amdgcn_cvt_pkrtz(fmaf((float)hi.x, minus, a), fmaf((float)hi.y, minus, b)));
+    const f2 z = {{fmaf((float)hi.x, minus, a) * 2048.0f, fmaf((float)hi.y, minus, b) * 2048.0f}};
+    lo = __builtin_convertvector(z, h2);
 }}
 // the largest of the four lanes r, r + 16, r + 32, r + 48: the swaps leave one half of a pair in each operand
 static __device__ __forceinline__ float four_max(float x) {{
@@ -706,7 +741,7 @@ extern "C" __global__ __launch_bounds__({bounds}) void {name}(const float* __res
         const float up = copysignf(__uint_as_float((u32)(14 - e + 127) << 23), scale);
         back[a] = __uint_as_float((u32)(e - 14 + 127) << 23) * l2;
         #pragma unroll
-        for (u32 i = 0; i < {Q4 // 2}u; ++i) halves(f[2u * i] * up, f[2u * i + 1u] * up, minus, q1[a][i >> 2].p[i & 3u], q2[a][i >> 2].w[i & 3u]);
+        for (u32 i = 0; i < {Q4 // 2}u; ++i) halves(f[2u * i] * up, f[2u * i + 1u] * up, minus, q1[a][i >> 2].p[i & 3u], q2[a][i >> 2].p[i & 3u]);
     }}
     f4 o[NQ][ND];
     float m[NQ], l[NQ];
@@ -751,17 +786,7 @@ extern "C" __global__ __launch_bounds__({bounds}) void {name}(const float* __res
         f4 s[NQ][4];
         #pragma unroll
         for (u32 u = 0; u < 4u; ++u) {{
-            #pragma unroll
-            for (u32 a = 0; a < NQ; ++a) s[a][u] = (f4){{0.f, 0.f, 0.f, 0.f}};
-            #pragma unroll
-            for (u32 i = 0; i < NK; ++i) {{
-                const h8 k8 = widen({half});
-                #pragma unroll
-                for (u32 a = 0; a < NQ; ++a) {{
-                    s[a][u] = MFMA16(k8, q2[a][i].v, s[a][u]);
-                    s[a][u] = MFMA16(k8, q1[a][i].v, s[a][u]);
-                }}
-            }}
+            {scores}
         }}
         load_k(jn);
         const u32 at = j * 64u + 16u * g;
@@ -800,7 +825,7 @@ extern "C" __global__ __launch_bounds__({bounds}) void {name}(const float* __res
                 float z = __builtin_amdgcn_exp2f(fmaf(s[a][i >> 2][(i & 3u) + 1u], f, up));
                 if constexpr (edge) {{ p = at + i < see[a] ? p : 0.0f; z = at + i + 1u < see[a] ? z : 0.0f; }}
                 sum += p + z;
-                halves(p, z, minus, p1[a][i >> 3].p[(i & 7u) >> 1], p2[a][i >> 3].w[(i & 7u) >> 1]);
+                halves(p, z, minus, p1[a][i >> 3].p[(i & 7u) >> 1], p2[a][i >> 3].p[(i & 7u) >> 1]);
             }}
             l[a] += sum;
         }}
@@ -809,13 +834,13 @@ extern "C" __global__ __launch_bounds__({bounds}) void {name}(const float* __res
             const h8 v0 = widen(vr[dt].x, vr[dt].y), v1 = widen(vr[dt].z, vr[dt].w);
             #pragma unroll
             for (u32 a = 0; a < NQ; ++a) {{
-                f4 acc = (f4){{0.f, 0.f, 0.f, 0.f}};
-                acc = MFMA16(v0, p2[a][0].v, acc);
-                acc = MFMA16(v1, p2[a][1].v, acc);
+                f4 acc = (f4){{0.f, 0.f, 0.f, 0.f}}, low = acc;
+                low = MFMA16(v0, p2[a][0].v, low);
                 acc = MFMA16(v0, p1[a][0].v, acc);
+                low = MFMA16(v1, p2[a][1].v, low);
                 acc = MFMA16(v1, p1[a][1].v, acc);
                 #pragma unroll
-                for (u32 i = 0; i < 4u; ++i) o[a][dt][i] = fmaf(vs, acc[i], o[a][dt][i]);
+                for (u32 i = 0; i < 4u; ++i) o[a][dt][i] = fmaf(vs, fmaf(low[i], LOW, acc[i]), o[a][dt][i]);
             }}
         }}
         load_v(jn);
@@ -843,7 +868,7 @@ extern "C" __global__ __launch_bounds__({bounds}) void {name}(const float* __res
             const float turn = kept ? back[a] : __builtin_nanf("");
             f4 acc = (f4){{0.f, 0.f, 0.f, 0.f}};
             #pragma unroll
-            for (u32 i = 0; i < {Q4}u; ++i) acc = MFMA32(kt[i], (float)q1[a][i >> 3].e[i & 7u] + (float)q2[a][i >> 3].e[i & 7u], acc);
+            for (u32 i = 0; i < {Q4}u; ++i) acc = MFMA32(kt[i], fmaf((float)q2[a][i >> 3].e[i & 7u], LOW, (float)q1[a][i >> 3].e[i & 7u]), acc);
             float mx = NINF;
             #pragma unroll
             for (u32 i = 0; i < 4u; ++i) {{

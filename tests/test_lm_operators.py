@@ -867,6 +867,62 @@ def test_cache_attention_adds_up_many_small_weights(gap):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("tiles,waves,splits", [(1, 4, 1), (2, 4, 1), (1, 8, 1), (1, 4, 3)])
+@pytest.mark.parametrize("gap", [18.3, 26.7, 38.45])
+def test_cache_attention_keeps_weights_far_below_the_largest(gap, tiles, waves, splits, monkeypatch):
+    """2^18 tokens of weights around 2^-gap, no power of two among them, behind some of weight 1, one in each wavefront's first block, whose
+    values are 0: all of the result is the others'.  A weight is off by 2^-22 of itself for the two 16-bit floats, or 2^-51 of the largest;
+    by 2 roundings of its score; each partial sum by a rounding, of at most 64 + a wavefront's n / 256 blocks."""
+    require_gpu()
+    monkeypatch.setattr(HIPLM, "attend_tiles", staticmethod(lambda *a: tiles))
+    monkeypatch.setattr(HIPLM, "attend_waves", staticmethod(lambda *a: waves))
+    monkeypatch.setattr(HIPLM, "attend_splits", staticmethod(lambda *a: splits))
+    rng = np.random.default_rng(44)
+    n, d = 1 << 18, 32
+    k, v = np.zeros((1, n, d), f32), (1 + 0.25 * rng.standard_normal((1, n, d))).astype(f32)
+    k[0, :, 3] = -np.repeat(rng.uniform(0, 0.5, n // 64), 64)                 # scores down to -1, the same in a block
+    for s in range(splits):
+        for block in range(n // 64 * s // splits, n // 64 * s // splits + waves):
+            k[0, block * 64 + 7, 3] = gap * math.log(2) / 2
+            v[0, block * 64 + 7] = 0
+    q = np.zeros((1, 1, d), f32)
+    q[0, 0, 3] = 2.0
+    cache = filled(1, n, 1, d, (k[:, :-1], v[:, :-1]))
+    cache.write(hip_tensor(k[:, -1:]), hip_tensor(v[:, -1:]))
+    y = cache.attend(hip_tensor(q), 1.0).numpy().reshape(d)
+    kk, vv = held(k[0][:, None], n)[:, 0].astype(np.float64), held(v[0][:, None], n)[:, 0].astype(np.float64)
+    w = np.exp(2 * (kk[:, 3] - kk[:, 3].max()))
+    want, small = w @ vv / w.sum(), w[w < 0.5].sum()
+    assert (w >= 0.5).sum() == splits * waves and small <= 4 * n * 2.0 ** -gap
+    tol = np.abs(vv).max() / w.sum() * (small * (2.0 ** -22 + 2 * (gap + 2) * EPS + (64 + n / 256) * EPS) + n * 2.0 ** -51)
+    within(y, want, tol, f"weights of 2^-{gap}")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tiles,waves,splits", [(1, 4, 1), (2, 4, 1), (1, 8, 1), (1, 4, 3)])
+@pytest.mark.parametrize("d", [32, 64])
+def test_cache_attention_of_a_query_with_one_huge_element(d, tiles, waves, splits, monkeypatch):
+    """An element 2^30 times the others, in a column where the keys are nothing: the others make the scores.  They are off by 2^-22 of
+    themselves (in the common bound) or 2^-50 of the largest, 2^-20 here."""
+    require_gpu()
+    monkeypatch.setattr(HIPLM, "attend_tiles", staticmethod(lambda *a: tiles))
+    monkeypatch.setattr(HIPLM, "attend_waves", staticmethod(lambda *a: waves))
+    monkeypatch.setattr(HIPLM, "attend_splits", staticmethod(lambda *a: splits))
+    rng = np.random.default_rng(45)
+    n = 400
+    k, v = rows_of(rng, 1, n, d)
+    k[:, :, 5] = 0
+    q = rng.standard_normal((1, 1, d)).astype(f32)
+    q[0, 0, 5] = 2.0 ** 30
+    cache = filled(1, n, 1, d, (k[:, :-1], v[:, :-1]))
+    cache.write(hip_tensor(k[:, -1:]), hip_tensor(v[:, -1:]))
+    kk, vv = (held(a[0].reshape(n, 1, d), n // 64 * 64) for a in (k, v))
+    want, tol = attended(q.reshape(1, 1, d), kk, vv, n - 1, 0.2, 1)
+    tol = tol + np.abs(vv).max() * 2 * np.abs(kk).sum(2).max() * 0.2 * 2.0 ** (30 - 50)
+    within(cache.attend(hip_tensor(q), 0.2).numpy().reshape(1, 1, d), want, tol)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tiles,waves,splits", [(1, 4, 1), (2, 4, 1), (1, 8, 1), (1, 4, 3)])
 @pytest.mark.parametrize("G,later", [(1, 0.0), (3, 0.0), (1, 1e-36)])
 def test_cache_attention_beside_a_block_of_zero_keys(G, later, tiles, waves, splits, monkeypatch):
     """Scores far below zero in the first block, keys of nothing (or next to it) in the second: a query that sees none of the second is

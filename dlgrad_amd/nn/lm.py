@@ -58,6 +58,16 @@ def rotary_frequencies(rotated: int, base: float = 10000.0, scaling: str | None 
     return f, 1.0
 
 
+def _copied(b: Buffer | None) -> Buffer | None:
+    """A copy on the hip device."""
+    if b is None:
+        return None
+    from dlgrad_amd.runtime.hip import alloc
+    own = Buffer.fresh(alloc(b.numel), b.shape, Device.HIP)
+    own.copy_(b)
+    return own
+
+
 def _on_hip(b: Buffer) -> bool:
     return b.device is Device.HIP and b.ptr.__class__ is not HostScalar
 
@@ -156,6 +166,8 @@ class Rotary:
             out = self._launch([(x.data, h, h * d) for x, h in zip(xs, heads)], shapes[0], back, p, s0)
         else:
             out = [self._launch([(x.data, h, h * d)], s, back, p, s0)[0] for x, h, s in zip(xs, heads, shapes)]
+        if any(x.requires_grad for x in xs):                            # (the backward pass turns by the angles of this call, wherever the tensors have moved by then)
+            p, s0 = _copied(p), _copied(s0)
         return [ops.Rotary.execute(x, turned=y, rope=self, n_head=h, geometry=s, positions=p, start=s0, back=back) if x.requires_grad else Tensor(y)
                 for x, y, h, s in zip(xs, out, heads, shapes)]
 

@@ -691,7 +691,7 @@ class SelfAttentionQKV(OP):
 
 class Rotary(OP):
     """A tensor turned by rotary positions (nn.Rotary), which the caller has computed: queries and keys turn in one launch and are
-    one node each.  The map is linear; backward is its transpose, the same kernel with the angles reversed."""
+    one node each.  positions and start are the node's own copies.  The map is linear; backward is its transpose, the same kernel with the angles reversed."""
 
     def forward(self, x: Buffer, turned: Buffer, rope, n_head: int, geometry: tuple, positions: Buffer | None, start: Buffer | None, back: bool) -> Buffer:
         self.rope, self.how = rope, (n_head, geometry, positions, start, back)

@@ -207,6 +207,26 @@ def test_rotary_gradient(layout):
     assert abs((at(step) - at(-step)) / (2 * step) - norm) <= 1e-5 * norm       # linear: differences are exact but for the gradient's own roundings
 
 
+@pytest.mark.parametrize("device", ["cpu", pytest.param("hip", marks=pytest.mark.gpu)])
+def test_rotary_gradient_turns_back_by_the_positions_of_its_forward(device):
+    """Positions and starts that have moved on by the time of the backward pass."""
+    if device == "hip":
+        require_gpu()
+    rng = np.random.default_rng(14)
+    rope = nn.Rotary(8, device=device)
+    q, k, gq, gk = (rng.standard_normal((2, 3, n)).astype(f32) for n in (16, 8, 16, 8))
+    p, s0 = rng.integers(0, 50, (2, 3)).astype(f32), np.array([[4], [9]], f32)
+    make = lambda a, **kw: Tensor(np.array(a), device=device, **kw)              # noqa: E731
+    qt, kt, pt, st = make(q, requires_grad=True), make(k, requires_grad=True), make(p), make(s0)
+    y, z = rope.pair(qt, kt, 2, 1, positions=pt, start=st)
+    loss = (y * make(gq)).sum() + (z * make(gk)).sum()
+    for t in (pt, st):
+        t.data.copy_(make(np.full(t.shape, 31.0, f32)).data)
+    loss.backward()
+    within(qt.grad.numpy(), turned(gq, 2, rope, p + s0, True), turned_tol(gq, rope), "dq")
+    within(kt.grad.numpy(), turned(gk, 1, rope, p + s0, True), turned_tol(gk, rope), "dk")
+
+
 def test_rotary_composed_of_existing_ops_on_the_cpu():
     rng = np.random.default_rng(1)
     for layout in ("half", "interleaved"):

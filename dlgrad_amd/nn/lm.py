@@ -380,8 +380,9 @@ def adjust_logits(logits: Tensor, history: Tensor | None = None, lengths: Tensor
     presence + frequency * c; the three are numbers, or tensors with one per row (taken as they are).  Then bias, (V,) or
     (B, V), is added, and tokens that hidden, (V,) or (B, V), marks (> 0: a grammar's mask) become -inf whatever they were; a row
     may be hidden whole.  One launch on the hip device; elsewhere on the host, from the downloaded logits."""
-    if logits.requires_grad or (bias is not None and bias.requires_grad):
-        _no_tape("adjust_logits")
+    for t in (logits, repetition, presence, frequency, bias):
+        if t.__class__ is Tensor and t.requires_grad:
+            _no_tape("adjust_logits")
     x, h, n = logits.data, None if history is None else history.data, None if lengths is None else lengths.data
     b, m = None if bias is None else bias.data, None if hidden is None else hidden.data
     r, p, f = (t.data if t.__class__ is Tensor else t for t in (repetition, presence, frequency))

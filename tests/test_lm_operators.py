@@ -388,6 +388,17 @@ def test_adjust_logits_on_the_cpu_and_refusals():
         nn.adjust_logits(Tensor(x, requires_grad=True))
 
 
+@pytest.mark.parametrize("which", ["repetition", "presence", "frequency", "bias"])
+def test_adjust_logits_refuses_to_stop_a_gradient(which):
+    x, h = Tensor(np.ones((2, 3), f32)), Tensor(np.zeros((2, 1), f32))
+    t = Tensor(np.ones((2, 3) if which == "bias" else (2, 1), f32), requires_grad=True)
+    with pytest.raises(ValueError, match="no gradient"):
+        nn.adjust_logits(x, h, **{which: t})
+    with nn.inference():
+        nn.adjust_logits(x, h, **{which: t})
+    nn.adjust_logits(x, h, **{which: t.detach()})
+
+
 # ================================================================ the 8-bit cache
 def held(rows, whole):
     """rows (n, H, d) as the cache stands for them: the first `whole` tokens in blocks of 64 per head, scale = max / 127 in fp32,

@@ -454,12 +454,6 @@ class Buffer:
         outs = _dispatch_table[(CustomOps.ROTARY, parts[0][0].device)](parts=parts, **kw)
         return [p[0] for p in parts] if kw.get("inplace") else [p[0]._like(o) for p, o in zip(parts, outs)]
 
-    def adjust_logits(self, history: "Buffer | None", lengths: "Buffer | None", penalties: tuple, bias: "Buffer | None",
-                      hidden: "Buffer | None") -> "Buffer":
-        """self: (B, V) logits; penalties for the tokens of the history, a bias and a mask, as nn.adjust_logits describes them."""
-        return self._like(self._dispatch(CustomOps.ADJUST_LOGITS, logits=self, history=history, lengths=lengths, penalties=penalties,
-                                         bias=bias, hidden=hidden))
-
     def log_softmax(self, dim: int) -> "Buffer":
         return self._unary(CustomOps.LOG_SOFTMAX, dim=dim)
 

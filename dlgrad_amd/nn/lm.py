@@ -393,8 +393,7 @@ def adjust_logits(logits: Tensor, history: Tensor | None = None, lengths: Tensor
         return _result(x._like(plan(x, h, n, (r, p, f), b, m)))
     _check_adjust(logits, history, lengths, repetition, presence, frequency, bias, hidden)
     if ops.FUSED and logits.device is Device.HIP:
-        from dlgrad_amd.runtime.hip_lm import HIPLM
-        plan = HIPLM.logits_plan(x, h, n, (r, p, f), b, m)
+        plan = _dispatch_table[(CustomOps.ADJUST_LOGITS, Device.HIP)](x, h, n, (r, p, f), b, m)
         if len(_adjust_plans) >= 1024:                                  # (a workload whose shapes never repeat)
             _adjust_plans.clear()
         _adjust_plans[key] = plan

@@ -305,14 +305,10 @@ class HIPLM:
 
     @staticmethod
     @dispatcher.register(CustomOps.ADJUST_LOGITS, Device.HIP)
-    def adjust_logits(logits: Buffer, history: Buffer | None, lengths: Buffer | None, penalties: tuple, bias: Buffer | None, hidden: Buffer | None) -> DevicePtr:
-        """logits (B, V); history (B, L); lengths B; penalties: (repetition, presence, frequency), each a float or a Buffer of B;
-        bias and hidden: V or (B, V)."""
-        return HIPLM.logits_plan(logits, history, lengths, penalties, bias, hidden)(logits, history, lengths, penalties, bias, hidden)
-
-    @staticmethod
     def logits_plan(logits: Buffer, history: Buffer | None, lengths: Buffer | None, penalties: tuple, bias: Buffer | None, hidden: Buffer | None):
-        """The checks of a call, which depend on shapes alone, and run(the same arguments) -> pointer for every call that agrees in them."""
+        """The checks of a call, which depend on shapes alone, and run(the same arguments) -> pointer for every call that agrees in them.
+        logits (B, V); history (B, L); lengths B; penalties: (repetition, presence, frequency), each a float or a Buffer of B;
+        bias and hidden: V or (B, V)."""
         pen = [p if isinstance(p, Buffer) else None for p in penalties]
         _on_device("adjust_logits", logits=logits, history=history, lengths=lengths, bias=bias, hidden=hidden, repetition=pen[0], presence=pen[1], frequency=pen[2])
         if logits.ndim != 2 or logits.shape[1] > EXACT_WHOLE:

@@ -43,6 +43,8 @@ def rotary_frequencies(rotated: int, base: float = 10000.0, scaling: str | None 
         raise ValueError(f"rotary: no scaling {scaling!r} (None, 'linear', 'base' or 'parts')")
     if rotated < 2 or rotated % 2 or not base > 0 or not math.isfinite(base) or not factor > 0 or not math.isfinite(factor):
         raise ValueError(f"rotary: {rotated} elements, base {base}, factor {factor}")
+    if scaling is None and factor != 1.0:
+        raise ValueError(f"rotary: a factor of {factor} and no scaling to take it")
     if scaling == "base":
         if rotated == 2:
             raise ValueError("rotary: one pair has no slowest one apart from the fastest: scaling 'base' needs four elements")

@@ -271,6 +271,13 @@ def test_rotary_refusals():
             call()
 
 
+def test_rotary_refuses_a_factor_without_a_scaling():
+    for call in (lambda: nn.Rotary(8, factor=8.0, device="cpu"), lambda: nn.rotary_frequencies(8, factor=0.5)):
+        with pytest.raises(ValueError, match="no scaling"):
+            call()
+    assert nn.Rotary(8, factor=1, trained=64, device="cpu").gain == 1.0
+
+
 def test_rotary_runtime_refuses_what_does_not_fit():
     """Host checks of the launch, before any device is touched."""
     class Ptr:

@@ -354,7 +354,7 @@ def _check_adjust(logits, history, lengths, repetition, presence, frequency, bia
     if logits.ndim != 2:
         raise ValueError(f"adjust_logits: logits {logits.shape} are not (B, V)")
     for name, p in (("repetition", repetition), ("presence", presence), ("frequency", frequency)):
-        if not isinstance(p, Tensor) and (not math.isfinite(p) or (name == "repetition" and not p > 0)):
+        if not isinstance(p, Tensor) and not (1e-38 if name == "repetition" else -3.4e38) <= p <= 3.4e38:      # (what fp32 holds, not a denormal)
             raise ValueError(f"adjust_logits: {name} = {p}")
     given = [t for t in (history, lengths, repetition, presence, frequency, bias, hidden) if isinstance(t, Tensor)]
     if any(t.device is not logits.device or t.data.is_host_scalar for t in given):

@@ -395,6 +395,14 @@ def test_adjust_logits_on_the_cpu_and_refusals():
         nn.adjust_logits(Tensor(x, requires_grad=True))
 
 
+def test_adjust_logits_refuses_numbers_that_fp32_does_not_hold():
+    x, h = Tensor(np.ones((1, 3), f32)), Tensor(np.zeros((1, 1), f32))
+    for bad in (dict(repetition=1e-50), dict(repetition=1e300), dict(presence=1e39), dict(frequency=-1e39), dict(presence=float("nan")), dict(frequency=float("-inf"))):
+        with pytest.raises(ValueError, match=next(iter(bad))):
+            nn.adjust_logits(x, h, **bad)
+    nn.adjust_logits(x, h, repetition=2, presence=-3, frequency=np.float32(0.5))
+
+
 @pytest.mark.parametrize("which", ["repetition", "presence", "frequency", "bias"])
 def test_adjust_logits_refuses_to_stop_a_gradient(which):
     x, h = Tensor(np.ones((2, 3), f32)), Tensor(np.zeros((2, 1), f32))

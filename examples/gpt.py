@@ -115,7 +115,8 @@ class KVCache:
 
 
 class KVCache8:
-    """The same for GPTConfig(cache="int8"): nn.QuantizedKVCache, a quarter of the memory.  lengths: a (batch, 1) device tensor
+    """The same for GPTConfig(cache="int8"): nn.QuantizedKVCache.  It takes less memory for a block_size of 192 or more (heads of 32 n elements),
+    38 % at 1024; at the default 128 it takes 125 %.  lengths: a (batch, 1) device tensor
     with the number of tokens held, if the caller keeps one."""
 
     quantized = True

@@ -1101,6 +1101,15 @@ def test_cache_steps_in_a_captured_graph():
 
 
 @pytest.mark.gpu
+def test_cache_takes_the_memory_that_is_documented():
+    """Percent of the bytes of two fp32 stores of the same tokens."""
+    require_gpu()
+    for tokens, d, percent in ((128, 32, 125), (128, 64, 125), (192, 64, 92), (1024, 64, 37.5), (32768, 128, 25.5), (1024, 40, 60), (32768, 40, 41), (32768, 16, 51)):
+        cache = nn.QuantizedKVCache(2, tokens, 3, d)
+        assert abs(100 * cache.nbytes / (2 * 3 * tokens * 8 * d) - percent) < 0.6, (tokens, d)
+
+
+@pytest.mark.gpu
 def test_cache_of_several_layers_and_shared_lengths():
     require_gpu()
     rng = np.random.default_rng(3)

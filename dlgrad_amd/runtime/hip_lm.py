@@ -191,15 +191,17 @@ class HIPLM:
         """Tiles of 16 query rows that a wavefront of the 8-bit attention holds.  Two share the widening of the codes (4 x 12 heads of 64,
         512 rows after 4096 tokens: 77 us against 85; 8 x 12 heads, 1024 after 1024: 129 against 135) but halve the
         workgroups, of which there should be three for every compute unit (the same with 256 rows: 53 us against 50); heads wider
-        than 64 have no registers for them (2 x 8 heads of 128, 512 after 2048: 40.6 us both ways)."""
-        return 2 if width <= 64 and pairs * -(-rows // 32) >= 3 * compute_units else 1
+        than 64 have no registers for them (2 x 8 heads of 128, 512 after 2048: 40.6 us both ways).  Up to 16 rows are one tile
+        (64 x 12 heads of 64 over 2000 tokens, 16 rows: 37 us against 45; 32 rows: 50 against 47)."""
+        return 2 if width <= 64 and rows > 16 and pairs * -(-rows // 32) >= 3 * compute_units else 1
 
     @staticmethod
-    def attend_waves(tiles: int, blocks: int, width: int) -> int:
-        """Wavefronts of a workgroup of the 8-bit attention.  With one tile of query rows, eight halve the blocks that each goes through
+    def attend_waves(rows: int, blocks: int, width: int) -> int:
+        """Wavefronts of a workgroup of the 8-bit attention.  With one tile of 16 query rows, eight halve the blocks that each goes through
         (16 x 12 heads of 64 over 4096 tokens: 19.1 us against 23.1 with four); heads wider than 64 fill the registers with four
-        (4 x 8 heads of 128 over 8192: 22.5 us, 23.0 with eight), and so few blocks as four leave the others idle (5.7, 6.3 us)."""
-        return 8 if tiles == 1 and width <= 64 and blocks > 4 else 4
+        (4 x 8 heads of 128 over 8192: 22.5 us, 23.0 with eight), so few blocks as four leave the others idle (5.7, 6.3 us), and
+        rows that two tiles share have workgroups enough (64 x 12 heads of 64 over 2000 tokens, 32 rows: 47 us with four, 61 with eight)."""
+        return 8 if rows <= 16 and width <= 64 and blocks > 4 else 4
 
     @staticmethod
     def attend_streams(c: Cache8, tiles: int) -> bool:
@@ -234,7 +236,7 @@ class HIPLM:
             return lambda qa, la, ca, scale: alloc(0)
         nq = HIPLM.attend_tiles(rows, pairs, c.width, props()["compute_units"])
         tiles = -(-rows // (16 * nq))
-        waves = HIPLM.attend_waves(tiles, c.blocks, c.width)
+        waves = HIPLM.attend_waves(rows, c.blocks, c.width)
         splits = HIPLM.attend_splits(pairs * tiles, c.blocks, waves, props()["compute_units"])
         grid = pairs * tiles * splits
         if grid >= 2 ** 31 or pairs * rows >= 2 ** 31:

@@ -1231,6 +1231,17 @@ def test_splits_and_slices():
         assert items == 4 or B * -(-V // (256 * items)) >= 512
 
 
+def test_attention_forms_by_rows():
+    """No tile of query rows is all padding, and eight wavefronts come with one tile, as the kernels are made for."""
+    for pairs in (1, 96, 768, 5000):
+        for rows in (1, 2, 15, 16, 17, 31, 32, 33, 500):
+            for width in (32, 64, 128):
+                nq, waves = HIPLM.attend_tiles(rows, pairs, width, 256), HIPLM.attend_waves(rows, 40, width)
+                assert nq == 1 or rows > 16
+                assert waves == 4 or (nq == 1 and rows <= 16 and width <= 64)
+    assert HIPLM.attend_tiles(1, 768, 64, 256) == 1 and HIPLM.attend_waves(1, 40, 64) == 8 and HIPLM.attend_tiles(17, 768, 64, 256) == 2
+
+
 # ================================================================ in the GPT of the examples
 TINY = dict(vocab_size=33, block_size=96, n_layer=2, n_head=2, n_embd=64, batch_size=3)
 

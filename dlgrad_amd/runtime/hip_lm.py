@@ -298,10 +298,11 @@ class HIPLM:
     @staticmethod
     def adjust_items(B: int, V: int, compute_units: int) -> int:
         """Logits per thread of the adjustment: every block walks its row's whole history, so long slices of the vocabulary save
-        walks -- as long as there are two blocks for every compute unit (256 x 128256 logits, 4000 said: 59 us with 8, 52 with 16, 55
-        with 32; 32 x 128256, 300 said: 9.3, 9.7, 11.1)."""
-        for items in (16, 8):
-            if B * -(-V // (256 * items)) >= 2 * compute_units:
+        walks -- as long as there are blocks enough, four for every compute unit with 16 (32 x 128256 logits, 4000 said, 4 a unit: 10.1 us with 16,
+        10.4 with 8; 256 x 128256, 32 a unit: 47.3, 48.7; 16 x 128256, 300 said, 2 a unit: 7.0, 6.7; 64 x 50257, 3.3 a unit: 12.3, 11.0), two with 8
+        (32 x 50304, 3.1 a unit: 6.6 us with 8, 7.3 with 4; 8 x 50304, 0.8 a unit: 5.1, 4.6)."""
+        for items, blocks in ((16, 4), (8, 2)):
+            if B * -(-V // (256 * items)) >= blocks * compute_units:
                 return items
         return 4
 

@@ -1231,6 +1231,15 @@ def test_splits_and_slices():
         assert items == 4 or B * -(-V // (256 * items)) >= 512
 
 
+def test_adjust_items_by_blocks():
+    """Sixteen logits a thread from four blocks a compute unit on, eight from two."""
+    for B, V in ((1, 65), (8, 50304), (16, 128256), (32, 50304), (32, 128256), (64, 50257), (64, 32000), (100, 50257), (65535, 1)):
+        items = HIPLM.adjust_items(B, V, 256)
+        blocks = lambda n: B * -(-V // (256 * n))                          # noqa: E731
+        assert items == (16 if blocks(16) >= 1024 else 8 if blocks(8) >= 512 else 4), (B, V)
+    assert [HIPLM.adjust_items(B, V, 256) for B, V in ((8, 50304), (16, 128256), (64, 50257), (32, 128256))] == [4, 8, 8, 16]
+
+
 def test_attention_forms_by_rows():
     """No tile of query rows is all padding, and eight wavefronts come with one tile, as the kernels are made for."""
     for pairs in (1, 96, 768, 5000):

@@ -15,9 +15,10 @@ from dlgrad_amd.helpers import CustomOps
 from dlgrad_amd.runtime.hip import DevicePtr, _addr, _PlanCache, _upload, alloc, field_offset, kernel, launch, launch_out, props
 
 STREAM_BYTES = 1 << 28       # the Infinity Cache
-# elements from which rotary positions bypass the L2 caches (queries and keys of 16 x 1024 x 12 heads of 64, 2 x 50 MB: 33.7 us against 39.1, with
-# an addition of the two behind it 59.4 against 62.9; of 8 x 1024, 2 x 25 MB: 17.2 against 18.8, but 17.1 against 16.4 for inputs turned twice)
-ROTARY_STREAM_ELEMENTS = 1 << 23
+# elements from which rotary positions bypass the caches.  Queries and keys with an addition in front of each and one of both behind, against the
+# same through the caches: 16 x 128 x 4 heads of 32 (2^19 elements) 11.7 us, 11.4; 2 x 512 x 12 heads of 64 (1.5 2^20) 15.4, 15.8; 2 x 1024 18.5, 21.3; 4 x 1024
+# 30.8, 32.5; 8 x 1024 54.6, 53.3; 16 x 1024 105.7, 106.8; 32 x 1024 223, 231.  Alone, from inputs that no cache holds: 2 x 1024 7.1, 8.3; 8 x 1024 19.7, 21.7.
+ROTARY_STREAM_ELEMENTS = 1 << 20
 EXACT_WHOLE = 1 << 24        # whole numbers up to here are exact in fp32
 _rotary_plans: dict = _PlanCache()     # what a call looked at -> the launch that its checks ended in
 

@@ -172,6 +172,22 @@ def test_rotary_beyond_the_caches_has_the_same_bits(layout, monkeypatch):
 
 
 @pytest.mark.gpu
+def test_rotary_by_size_has_the_bits_of_its_pieces():
+    """Enough elements to bypass the caches, against pieces that do not."""
+    require_gpu()
+    from dlgrad_amd.runtime import hip_lm
+    rng = np.random.default_rng(15)
+    q, k = (rng.standard_normal((1, 700, 12 * 64)).astype(f32) for _ in range(2))
+    assert q.size + k.size >= hip_lm.ROTARY_STREAM_ELEMENTS > 2 * q[:, :300].size
+    rope = nn.Rotary(64)
+    got = [t.numpy() for t in rope.pair(hip_tensor(q), hip_tensor(k), 12)]
+    for at in range(0, 700, 300):
+        rows = slice(at, at + 300)
+        for a, b in zip(got, rope.pair(hip_tensor(q[:, rows]), hip_tensor(k[:, rows]), 12, start=hip_tensor([[at]]))):
+            same(a[:, rows], b.numpy())
+
+
+@pytest.mark.gpu
 def test_rotary_of_unaligned_views_and_of_nothing():
     require_gpu()
     rng = np.random.default_rng(2)

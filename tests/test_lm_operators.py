@@ -352,6 +352,28 @@ def test_adjust_logits(B, V, L):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("B,V,L,items", [(3, 701, 66000, 4), (24, 50257, 9, 8), (24, 50256, 66000, 8), (24, 50257, 66000, 8), (100, 50257, 70, 16), (100, 50256, 66000, 16), (100, 50257, 66000, 16)])
+def test_adjust_logits_in_every_form(B, V, L, items):
+    """8 and 16 logits a thread with and without 16-byte accesses, and counters of 32 bits for long histories; bounds as above."""
+    require_gpu()
+    assert HIPLM.adjust_items(B, V, 256) == items
+    rng = np.random.default_rng(L + B)
+    x = (4 * rng.standard_normal((B, V))).astype(f32)
+    history = np.floor(rng.random((B, L), dtype=f32) ** 3 * (V + 2)).astype(f32) - 1              # from -1 to V
+    n = rng.integers(0, L + 1, B)
+    n[0] = L
+    history[0] = V - 1                                                      # one token, more often than 16 bits count
+    bias = rng.standard_normal(V).astype(f32)
+    want = x.astype(np.float64)
+    for b in range(B):
+        ids = history[b, :n[b]]
+        c = np.bincount(ids[(ids >= 0) & (ids < V)].astype(np.int64), minlength=V)
+        want[b] = np.where(c > 0, np.where(want[b] > 0, want[b] / f32(1.3), want[b] * f32(1.3)) - (float(f32(0.2)) + float(f32(0.1)) * c), want[b])
+    y = nn.adjust_logits(hip_tensor(x), hip_tensor(history), hip_tensor(n.reshape(B, 1)), 1.3, 0.2, 0.1, hip_tensor(bias))
+    within(y.numpy(), want + bias, 5 * EPS * (np.abs(x).max() * 2 + 1 + 0.1 * L + np.abs(bias).max()))
+
+
+@pytest.mark.gpu
 def test_adjust_logits_masks_and_special_values():
     require_gpu()
     x = np.array([[1.0, np.nan, np.inf, -np.inf, -2.0, 3.4e38, -3.4028235e38, 0.0]], f32).repeat(3, 0)
@@ -594,6 +616,24 @@ def test_cache_attention_in_every_form(B, H, G, d, n, T, cap, tiles, waves, spli
     if n % 64 and T > 64:
         n = n // 64 * 64
     test_cache_attention(B, H, G, d, n, T, cap)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("H,d", [(1, 192), (2, 161), (1, 224), (2, 200)])
+def test_cache_of_wide_heads(H, d):
+    test_cache_holds_the_same_however_the_tokens_arrive(H, d)
+    test_cache_attention(1, H, 2, d, 200, 3, 256)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("splits,stream", [(1, True), (3, False), (2, True)])
+@pytest.mark.parametrize("d", [96, 130, 192, 224, 256])
+def test_cache_attention_of_wide_heads_in_every_form(d, splits, stream, monkeypatch):
+    """Parts joined and loads past the caches, which long caches of such heads take."""
+    require_gpu()
+    monkeypatch.setattr(HIPLM, "attend_splits", staticmethod(lambda *a: splits))
+    monkeypatch.setattr(HIPLM, "attend_streams", staticmethod(lambda *a: stream))
+    test_cache_attention(1, 2, 3, d, 300, 21, 512)
 
 
 @pytest.mark.gpu

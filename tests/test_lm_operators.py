@@ -243,6 +243,35 @@ def test_rotary_gradient_turns_back_by_the_positions_of_its_forward(device):
     within(kt.grad.numpy(), turned(gk, 1, rope, p + s0, True), turned_tol(gk, rope), "dk")
 
 
+@pytest.mark.gpu
+def test_rotary_gradient_in_a_captured_step_follows_its_start():
+    """The copies of the positions are part of the step: each replay turns back by the start it turned by."""
+    require_gpu()
+    if hip.COMPILE_ONLY:
+        return
+    rng = np.random.default_rng(16)
+    rope = nn.Rotary(8)
+    q, k, gq, gk = (rng.standard_normal((2, 3, n)).astype(f32) for n in (16, 8, 16, 8))
+    qt, kt, gqt, gkt, st = hip_tensor(q, True), hip_tensor(k, True), hip_tensor(gq), hip_tensor(gk), hip_tensor([[0], [0]])
+
+    def step():
+        qt.grad = kt.grad = None
+        y, z = rope.pair(qt, kt, 2, 1, start=st)
+        loss = (y * gqt).sum() + (z * gkt).sum()
+        st.data.copy_((st + 5.0).data)                                       # the next call's
+        loss.backward()
+        return y
+    run = hip.CapturedStep(step)
+    p = np.arange(3) + np.zeros((2, 1))
+    for i in range(6):
+        y = run().numpy()
+        within(y, turned(q, 2, rope, p + 5 * i), turned_tol(q, rope), f"step {i}")
+        within(qt.grad.numpy(), turned(gq, 2, rope, p + 5 * i, True), turned_tol(gq, rope), f"dq of step {i}")
+        within(kt.grad.numpy(), turned(gk, 1, rope, p + 5 * i, True), turned_tol(gk, rope), f"dk of step {i}")
+        rope(hip_tensor(q), 2).numpy()                                        # work of its own between the replays
+    run.close()
+
+
 def test_rotary_composed_of_existing_ops_on_the_cpu():
     rng = np.random.default_rng(1)
     for layout in ("half", "interleaved"):

@@ -269,6 +269,7 @@ static __device__ __forceinline__ void cache8_extent(const float* __restrict__ l
     n = c >= (float)T ? T : c > 0.0f ? (u32)c : 0u;
     n = min(n, cap - len);
 }
+#define CACHE8_MARKS 32u                                                    // words from one head's marks to the next's
 // Whether a tail that says `mark` keeps the first `rows` (1 .. 63) rows of block blk: a mark is 64 * block + the rows that lie there.
 static __device__ __forceinline__ bool cache8_kept(u32 mark, u32 blk, u32 rows) {
     return mark >= blk * 64u + rows && mark <= blk * 64u + 64u;
@@ -316,7 +317,9 @@ def cache8_write_kernel(DP: int, vec: bool) -> tuple[str, str, str]:
     A call may be followed by one that starts at a smaller length than it ended at, or at its own again.  Both tails together hold what
     that takes while the call touches two blocks; one that completes more leaves the rows of the blocks between nowhere in fp32, and
     where it ends in the tail that it started in, those of its first block neither.  Each tail's mark says what lies there
-    (cache8_kept), and rows that are not there are NaN to whoever needs them.
+    (cache8_kept), and rows that are not there are NaN to whoever needs them.  The marks of a head have a line of memory to
+    themselves, because workgroups of different dies write them, and are waited for after the rows (8 x 12 heads of 64, a token: 3.8 us; with
+    neighbours in a line 4.1, waited for with the lengths 4.2; without marks 3.4).
 
     One workgroup of 512 threads per (block of 64, head, sequence), a thread per four columns of a row (DP / 32 times).  With 256 a
     launch of few workgroups, which is one pass over the code, takes longer (2 x 12 heads of 64, 512 tokens: 6.7 us against 5.4),
@@ -380,15 +383,36 @@ extern "C" __global__ __launch_bounds__({NT}) void {name}(const float* __restric
     const u32 t = threadIdx.x, lane = t & 63u, h = blockIdx.y, b = blockIdx.z;
     u32 len, n;
     const u64 bh = (u64)b * H + h, heads = (u64)gridDim.z * H;
-    const uint2 was = *reinterpret_cast<const uint2*>(marks + 2u * bh);       // (written by workgroup 0 alone, which alone goes by them)
+    const u32 was = marks[CACHE8_MARKS * bh + (lane & 1u)];                  // (written by workgroup 0 alone, which alone goes by them; a lane's load, since a scalar one would be waited for with the lengths)
     cache8_extent(lengths, counts, b, T, NB * 64u, len, n);
     const u32 total = len + n, first = len >> 6, last = total >> 6;         // last: the block that is not full afterwards
-    const u32 mine = first & 1u ? was.y : was.x, other = first & 1u ? was.x : was.y;
-    const bool lost = (len & 63u) && !cache8_kept(mine, first, len & 63u);      // the rows before this call are not in their tail
-    if (!n && blockIdx.x) return;
+    bool lost = false;                                                        // the rows before this call are not in their tail
+    u32 other = 0u;
+    auto look = [&]() {{
+        u32 m = was;
+        asm volatile("" : "+v"(m));                                             // (the marks are waited for here, not before the rows are loaded)
+        lost = (len & 63u) && !cache8_kept(__builtin_amdgcn_readlane(m, first & 1u), first, len & 63u);
+        other = __builtin_amdgcn_readlane(m, (first & 1u) ^ 1u);
+    }};
+    auto leave = [&]() {{                                                      // what the call leaves
+        if (h == 0u) wrote[b] = n;
+        const u32 f64 = first * 64u, l64 = last * 64u + (total & 63u);
+        // the first block's tail: what lay there, and the new rows where they are stored
+        u32 a = lost ? 0u : last == first ? l64 : last == first + 1u ? f64 + 64u : f64 + (len & 63u);
+        u32 o = other <= f64 ? other : 0u;                                  // the other one: not what a call before this one put there in its place
+        if (last > first) {{
+            if ((last - first) & 1u) o = l64;
+            else if (total & 63u) a = l64;
+        }}
+        *reinterpret_cast<uint2*>(marks + CACHE8_MARKS * bh) = first & 1u ? make_uint2(o, a) : make_uint2(a, o);
+    }};
+    if (!n) {{
+        if (blockIdx.x == 0u) {{ look(); if (t == 0u) leave(); }}
+        return;
+    }}
     const float* __restrict__ kh = k + (u64)b * T * kp + (u64)h * d;
     const float* __restrict__ vh = v + (u64)b * T * vp + (u64)h * d;
-    for (u32 pass = n ? 0u : 2u; pass < 2u; ++pass) {{
+    for (u32 pass = 0; pass < 2u; ++pass) {{
         const u32 blk = pass ? last : first + blockIdx.x;
         if (pass && (blockIdx.x != 0u || last == first || !(total & 63u))) break;       // (uniform over the workgroup)
         const bool full = blk < last;
@@ -418,7 +442,9 @@ extern "C" __global__ __launch_bounds__({NT}) void {name}(const float* __restric
         mk = wave_max(mk);
         mv = wave_max(mv);
         if (lane == 0u) {{ sk[t >> 6] = mk; sv[t >> 6] = mv; }}
+        if (!pass && blockIdx.x == 0u) look();
         __syncthreads();
+        if (!pass && blockIdx.x == 0u && t == 0u) leave();                      // (every thread has read the marks)
         // the rows as they came: needed while the block is not full (and again if the caller goes back into it)
         if (!full || (blk == first && last == first + 1u)) {{
             #pragma unroll
@@ -464,18 +490,6 @@ extern "C" __global__ __launch_bounds__({NT}) void {name}(const float* __restric
             }}
         }}
         __syncthreads();
-    }}
-    if (blockIdx.x == 0u && h == 0u && t == 0u) wrote[b] = n;
-    if (blockIdx.x == 0u && t == 0u) {{                                     // (the passes' barriers lie after every thread's read of the marks)
-        const u32 f64 = first * 64u, l64 = last * 64u + (total & 63u);
-        // the first block's: what lay there, and the new rows where they were stored
-        u32 a = lost ? 0u : last == first ? l64 : last == first + 1u ? f64 + 64u : f64 + (len & 63u);
-        u32 o = other <= f64 ? other : 0u;                                  // the other one's: not what a call before this one put there in its place
-        if (last > first) {{
-            if ((last - first) & 1u) o = l64;
-            else if (total & 63u) a = l64;
-        }}
-        *reinterpret_cast<uint2*>(marks + 2u * bh) = first & 1u ? make_uint2(o, a) : make_uint2(a, o);
     }}
 }}
 """
@@ -531,7 +545,7 @@ def cache8_read_kernel(DP: int) -> tuple[str, str, str]:
     __syncthreads();
     const float* __restrict__ tk = tail_k + (((u64)(blk & 1u) * heads + bh) * 64u) * DP;
     const float* __restrict__ tv = tail_v + (((u64)(blk & 1u) * heads + bh) * 64u) * DP;
-    const bool lost = blk == last && (total & 63u) && !cache8_kept(marks[2u * bh + (blk & 1u)], blk, total & 63u);
+    const bool lost = blk == last && (total & 63u) && !cache8_kept(marks[CACHE8_MARKS * bh + (blk & 1u)], blk, total & 63u);
     const u64 C = (u64)H * d;
     // four columns a thread (as many of them as there are)
     for (u32 i = t; i < 64u * {DP // 4}u; i += 256u) {{
@@ -854,7 +868,7 @@ extern "C" __global__ __launch_bounds__({bounds}) void {name}(const float* __res
         const float* __restrict__ tk = tail_k + (((u64)(last & 1u) * heads + bh) * 64u + 16u * tt) * DP;
         const float* __restrict__ tv = tail_v + (((u64)(last & 1u) * heads + bh) * 64u + 16u * tt) * DP;
         const u32 p0 = last * 64u + 16u * tt + 4u * g;                              // this lane's four tokens
-        const u32 mark = marks[2u * bh + (last & 1u)];
+        const u32 mark = marks[CACHE8_MARKS * bh + (last & 1u)];
         float kt[{Q4}], vt[ND][4];                                                  // (both on their way before the first is used)
         #pragma unroll
         for (u32 i = 0; i < {Q4}u; ++i) kt[i] = tk[r * DP + g * {Q4}u + i];

@@ -45,11 +45,11 @@ class Cache8:
         self.scales = Buffer.full((n, 2), 0.0, Device.HIP)
         # tails are read in whole blocks: columns beyond d, and rows not written yet, are zeros from the start
         self.tail_k, self.tail_v = (Buffer.full((2, batch * heads, K.CACHE8_BLOCK, self.width), 0.0, Device.HIP) for _ in range(2))
-        self.marks = Buffer.full((batch * heads, 2), 0.0, Device.HIP)         # (whole numbers of 32 bits, 0: nothing)
+        self.marks = Buffer.full((batch * heads, 32), 0.0, Device.HIP)        # (two whole numbers of 32 bits at the front of each row, 0: nothing)
 
     @property
     def nbytes(self) -> int:
-        """Bytes of codes, scales and tails (the marks are 8 more for each sequence and head)."""
+        """Bytes of codes, scales and tails (the marks are 128 more for each sequence and head)."""
         return self.kc.nbytes + self.vc.nbytes + self.scales.nbytes + self.tail_k.nbytes + self.tail_v.nbytes
 
 

@@ -326,7 +326,7 @@ def cache8_write_kernel(DP: int, vec: bool) -> tuple[str, str, str]:
     with 1024 many wait for each other's barriers (4 x 12 heads of 64, 4096 tokens: 37 us against 29, 4.4 TB/s).  Workgroup 0
     of a head completes the block that the call starts in and then stores the rows of the block it ends in, in this order,
     because both may use the same tail.  Bound by memory for long calls, 4 bytes read and 1 written per element; by its chain of
-    reads, reduction and stores for short ones (the token that completes 96 blocks: 5.1 us; one that completes none: 2.7)."""
+    reads, reduction and stores for short ones (the token that completes 96 blocks: 5.4 us; one that completes none: 3.0)."""
     name = f"cache8_write_d{DP}_{'v4' if vec else 'v1'}"
     NT = CACHE8_WRITE_THREADS
     IT = -(-16 * DP // NT)                     # four columns of a row per thread, so many times
@@ -608,9 +608,10 @@ def cache8_attend_kernel(DP: int, NQ: int = 1, W: int = 4, stream: bool = False)
     A workgroup of W wavefronts per (NQ tiles of one key head, split of the blocks); they are joined through LDS in
     wavefront order.  With one split y is written; else O, m and l go to `part` and cache8_join_kernel adds the splits up
     in their order.  Bound by memory while few query rows share a key head, 2 bytes per token and column (16 sequences up to 32768
-    tokens, 32 heads on 8 of 128: 132 us, 6.2 TB/s); with many by issue, some 295 vector and 32 matrix instructions a block of 64 and
-    tile of 16 rows, which do not overlap (4 x 12 heads of 64, 256 rows after 4096 tokens: 47 us, 285 TFLOP/s of the formula's
-    operations); with few blocks by chains of dependent reads (one block and a tail: 3.9 us)."""
+    tokens, 32 heads on 8 of 128: 132 us, 6.2 TB/s); with many by the issue of instructions, some 345 vector and 32 matrix ones a block of 64 and
+    tile of 16 rows (4 x 12 heads of 64, 256 rows after 4096 tokens: 47 us, 280 TFLOP/s of the formula's operations; the SIMDs issue vector
+    instructions in 66 % of the cycles, the matrix units are busy in 21 %); with few blocks by chains of dependent reads (one block and a
+    tail: 3.8 us)."""
     ND, NK, Q4 = DP // 16, DP // 32, DP // 4             # column tiles of V^T, k steps of a score, columns a lane feeds
     name = f"cache8_attend_d{DP}" + (f"_q{NQ}" if NQ > 1 else "") + (f"_w{W}" if W != 4 else "") + ("_nt" if stream else "")
     wide = Q4 % 16 == 0                                   # a lane's quarter of a key in 16-byte words, else in words of 8

@@ -190,34 +190,36 @@ class HIPLM:
     @staticmethod
     def attend_tiles(rows: int, pairs: int, width: int, compute_units: int) -> int:
         """Tiles of 16 query rows that a wavefront of the 8-bit attention holds.  Two share the widening of the codes (4 x 12 heads of 64,
-        512 rows after 4096 tokens: 77 us against 85; 8 x 12 heads, 1024 after 1024: 129 against 135) but halve the
-        workgroups, of which there should be three for every compute unit (the same with 256 rows: 53 us against 50); heads wider
-        than 64 have no registers for them (2 x 8 heads of 128, 512 after 2048: 40.6 us both ways).  Up to 16 rows are one tile
+        512 rows after 4096 tokens: 79 us against 88; 8 x 12 heads, 1024 after 1024: 123 against 133) but halve the
+        workgroups, of which there should be three for every compute unit (the same with 256 rows: 52 us against 47); heads wider
+        than 64 have no registers for them (2 x 8 heads of 128, 512 after 2048: 52 us against 35).  Up to 16 rows are one tile
         (64 x 12 heads of 64 over 2000 tokens, 16 rows: 37 us against 45; 32 rows: 50 against 47)."""
         return 2 if width <= 64 and rows > 16 and pairs * -(-rows // 32) >= 3 * compute_units else 1
 
     @staticmethod
     def attend_waves(rows: int, blocks: int, width: int) -> int:
         """Wavefronts of a workgroup of the 8-bit attention.  With one tile of 16 query rows, eight halve the blocks that each goes through
-        (16 x 12 heads of 64 over 4096 tokens: 19.1 us against 23.1 with four); heads wider than 64 fill the registers with four
-        (4 x 8 heads of 128 over 8192: 22.5 us, 23.0 with eight), so few blocks as four leave the others idle (5.7, 6.3 us), and
-        rows that two tiles share have workgroups enough (64 x 12 heads of 64 over 2000 tokens, 32 rows: 47 us with four, 61 with eight)."""
+        (16 x 12 heads of 64 over 4096 tokens: 20.9 us against 24.8 with four); heads wider than 64 fill the registers with four
+        (4 x 8 heads of 128 over 8192: 24.7 us, 25.5 with eight), few blocks leave the others idle (1 x 12 heads of 64, two blocks: 5.0 us with four, 5.3
+        with eight; four: 5.95, 5.75; six: 6.1, 5.8), and rows that two tiles share have workgroups enough (64 x 12 heads of 64 over 2000 tokens,
+        32 rows: 47 us with four, 61 with eight).  It does not look at the batch: with more workgroups than compute units four are ahead for short
+        caches (40 x 12 heads of 64 over 738 tokens: 13.1 us, 14.1 with eight)."""
         return 8 if rows <= 16 and width <= 64 and blocks > 4 else 4
 
     @staticmethod
     def attend_streams(c: Cache8, tiles: int) -> bool:
         """Whether the codes bypass the caches: they are read once by a call, and the cache as a whole, all layers of it, is larger than
-        the 256 MiB that a later step might find them in (16 x 8 heads of 128 over 32768 tokens, 1.07 GB: 171 us against 192;
-        16 x 12 heads of 64 over 8192, 0.2 GB, again and again: 43.0 us against 38.4)."""
+        the 256 MiB that a later step might find them in (16 x 8 heads of 128 over 32768 tokens, 1.07 GB: 168 us against 193;
+        4 x 8 heads, 0.27 GB: 53 against 59; 16 x 12 heads of 64 over 8192, 0.2 GB, again and again: 40.4 us against 35.7)."""
         return tiles == 1 and c.layers * (c.kc.nbytes + c.vc.nbytes) > STREAM_BYTES
 
     @staticmethod
     def attend_splits(groups: int, blocks: int, waves: int, compute_units: int) -> int:
         """Into how many parts the blocks of a sequence are cut when one part makes `groups` workgroups of `waves` wavefronts.  A wavefront
         takes 0.8 us for a block when there are few, the second launch that joins the parts 3.5 us and 0.1 us for each:
-        sqrt(blocks / 2) parts from 8 blocks a wavefront on (1 x 12 heads of 64 over 4096 tokens, four wavefronts: 18.0 us
-        with one part, 11.9 with 4, 12.0 with 16; 1 x 8 heads of 128 over 32768: 40 us with 8, 34 with 16, 37 with 32), and no more than
-        eight wavefronts for every compute unit (16 x 12 heads of 64 over 4096: 23.4 us with 2 parts, 27.1 with 8).  The length is
+        sqrt(blocks / 2) parts from 8 blocks a wavefront on (1 x 12 heads of 64 over 4096 tokens: 17.0 us with one part, 11.3 with 4, 11.1 with
+        8, 12.5 with 16; 1 x 8 heads of 128 over 32768: 35 us with 8, 30 with 16, 34 with 32), and no more than
+        eight wavefronts for every compute unit (16 x 12 heads of 64 over 4096: 19.4 us with one part, 25.0 with 2, 29.6 with 8).  The length is
         device data; the capacity stands for it."""
         if blocks < 8 * waves:
             return 1

@@ -519,18 +519,19 @@ extern "C" __global__ __launch_bounds__(256) void cache8_advance(float* __restri
 def cache8_read_kernel(DP: int) -> tuple[str, str, str]:
     """The values that the cache of one layer stands for, as fp32 k and v (B, N, H * d): code * scale for the tokens of full
     blocks, the rows themselves for those of the tail, zeros from position lengths[b] + counts[b] on (counts: rows written
-    since the lengths were advanced; `extra` for every sequence without them).  One workgroup per (block of 64, head,
+    since the lengths were advanced, of those there are; `extra` for every sequence without them).  One workgroup per (block of 64, head,
     sequence); the codes pass through LDS so that rows leave as rows.  Bound by memory (8 x 1024 tokens of 12 heads of 64: 11.3 us,
     5.6 TB/s)."""
     name = f"cache8_read_d{DP}"
     src = f"""{PRELUDE}{_CACHE8}{_cache8_layout(DP)}extern "C" __global__ __launch_bounds__(256) void {name}(const unsigned char* __restrict__ kc, const unsigned char* __restrict__ vc,
         const float* __restrict__ scales, const float* __restrict__ tail_k, const float* __restrict__ tail_v, const u32* __restrict__ marks,
-        const float* __restrict__ lengths, const float* __restrict__ counts, float* __restrict__ ko, float* __restrict__ vo,
+        const u32* __restrict__ wrote, const float* __restrict__ lengths, const float* __restrict__ counts, float* __restrict__ ko, float* __restrict__ vo,
         u32 N, u32 H, u32 d, u32 NB, u32 extra) {{
     __shared__ __attribute__((aligned(16))) u32 kt[DP * 16u], vt[DP * 16u];       // the block's bytes
     const u32 t = threadIdx.x, blk = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
     u32 len, n;
     cache8_extent(lengths, counts, b, extra, NB * 64u, len, n);
+    n = min(n, wrote[b]);
     const u32 total = len + n, last = total >> 6;
     const u64 bh = (u64)b * H + h, heads = (u64)gridDim.z * H, at = bh * NB + blk;
     const float s_k = blk < last ? scales[2u * at] : 0.0f, s_v = blk < last ? scales[2u * at + 1u] : 0.0f;
@@ -576,14 +577,15 @@ def cache8_read_kernel(DP: int) -> tuple[str, str, str]:
     }}
 }}
 """
-    return src, name, _fmt("P" * 10, "I" * 5)
+    return src, name, _fmt("P" * 11, "I" * 5)
 
 
 @cache
 def cache8_attend_kernel(DP: int, NQ: int = 1, W: int = 4, stream: bool = False) -> tuple[str, str, str]:
     """Attention of T new positions per sequence over the 8-bit cache of one layer, after their keys and values were written:
     y = softmax(q K^T * scale) V per query head, query t of sequence b at position lengths[b] + t seeing the positions up to its
-    own; `group` query heads share a key head.  q and y are (B, T, H * group * d).  A row beyond counts[b] gives zeros.
+    own; `group` query heads share a key head.  q and y are (B, T, H * group * d).  A row beyond counts[b], or beyond what the last write
+    brought, gives zeros.
 
     The codes are whole numbers of at most 127 and therefore exact in 16-bit floats, so the matrix units do the work:
     a query row is scaled by a power of two to at most 2^15 and held as two 16-bit floats an element, q' = q1 + q2 / 2^11: q1 the
@@ -699,7 +701,8 @@ struct Inside {{ static constexpr bool edge = false; }};
 struct Edge {{ static constexpr bool edge = true; }};
 extern "C" __global__ __launch_bounds__({bounds}) void {name}(const float* __restrict__ q, const unsigned char* __restrict__ kc,
         const unsigned char* __restrict__ vc, const float* __restrict__ scales, const float* __restrict__ tail_k, const float* __restrict__ tail_v,
-        const u32* __restrict__ marks, const float* __restrict__ lengths, const float* __restrict__ counts, float* __restrict__ y, float* __restrict__ part,
+        const u32* __restrict__ marks, const u32* __restrict__ wrote, const float* __restrict__ lengths, const float* __restrict__ counts, float* __restrict__ y,
+        float* __restrict__ part,
         u32 B, u32 T, u32 H, u32 group, u32 d, u32 NB, u32 tiles, u32 splits, u32 q_wide, float scale) {{
     __shared__ float so[W][16][DP + 4u];
     __shared__ float sm[W][16], sl[W][16];
@@ -726,6 +729,7 @@ extern "C" __global__ __launch_bounds__({bounds}) void {name}(const float* __res
     }}
     u32 len, n;
     cache8_extent(lengths, counts, b, T, NB * 64u, len, n);
+    n = min(n, wrote[b]);                                                       // (a query whose key was not written is a padded row)
     #pragma unroll
     for (u32 a = 0; a < NQ; ++a)
         #pragma unroll
@@ -940,7 +944,7 @@ extern "C" __global__ __launch_bounds__({bounds}) void {name}(const float* __res
     }}
 }}
 """
-    return src, name, _fmt("P" * 11, "I" * 9, "f")
+    return src, name, _fmt("P" * 12, "I" * 9, "f")
 
 
 CACHE8_MAX_SPLITS = 64      # what one wavefront joins: a lane per split

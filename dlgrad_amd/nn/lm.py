@@ -307,7 +307,7 @@ class QuantizedKVCache:
 
     def attend(self, q: Tensor, scale: float | None = None, layer: int = 0, counts: Tensor | None = None) -> Tensor:
         """q (B, T, n_head * head_dim): the queries of positions lengths[b] .., whose keys and values write() has stored; each sees
-        the positions up to its own.  scale: of the scores, head_dim ** -0.5 without one."""
+        the positions up to its own.  Rows beyond those that the last write brought, its counts included, are zeros.  scale: of the scores, head_dim ** -0.5 without one."""
         if q.requires_grad:
             _no_tape("QuantizedKVCache.attend")
         scale = self.head_dim ** -0.5 if scale is None else float(scale)
@@ -321,7 +321,7 @@ class QuantizedKVCache:
 
     def read(self, n: int, layer: int = 0, new: int = 0, counts: Tensor | None = None) -> tuple[Tensor, Tensor]:
         """(k, v), both (B, n, n_kv_head * head_dim): the values that the first n positions stand for, zeros where a sequence is
-        shorter.  new, or counts: rows that were written since the last advance() and belong to it."""
+        shorter.  new, or counts: rows that were written since the last advance() and belong to it, as many as there are."""
         k, v = self._run(CustomOps.CACHE8_READ, layer, counts, n=int(n), extra=self.capacity if counts is not None else int(new))
         shape = (self.batch, int(n), self.n_kv_head * self.head_dim)
         return _result(Buffer.fresh(k, shape, Device.HIP)), _result(Buffer.fresh(v, shape, Device.HIP))

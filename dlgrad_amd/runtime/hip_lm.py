@@ -245,7 +245,7 @@ class HIPLM:
         if grid >= 2 ** 31 or pairs * rows >= 2 ** 31:
             raise ValueError(f"cache8_attend: {pairs} heads of {rows} query rows exceed the grid")
         k, join = kernel(K.cache8_attend_kernel, c.width, nq, waves, HIPLM.attend_streams(c, tiles)), kernel(K.cache8_join_kernel, c.width) if splits > 1 else None
-        held = (c.kc.addr, c.vc.addr, _addr(c.scales), _addr(c.tail_k), _addr(c.tail_v), _addr(c.marks))
+        held = (c.kc.addr, c.vc.addr, _addr(c.scales), _addr(c.tail_k), _addr(c.tail_v), _addr(c.marks), _addr(c.wrote))
         sizes = (c.batch, T, c.heads, group, c.d, c.blocks, tiles, splits)
         wide = c.d % 4 == 0                                              # (then the rows of the queries are whole 16-byte items)
         n_part, join_grid, join_sizes = pairs * rows * splits * (c.width + 2), (pairs * rows + 3) // 4, (pairs * rows, T, c.heads, group, c.d, splits)
@@ -282,7 +282,7 @@ class HIPLM:
         k, v = alloc(size), alloc(size)
         if size:
             launch(kernel(K.cache8_read_kernel, c.width), (-(-n // K.CACHE8_BLOCK), c.heads, c.batch), 256, c.kc.addr, c.vc.addr, _addr(c.scales),
-                   _addr(c.tail_k), _addr(c.tail_v), _addr(c.marks), _addr(lengths), _addr(counts) if counts is not None else 0, k.addr, v.addr,
+                   _addr(c.tail_k), _addr(c.tail_v), _addr(c.marks), _addr(c.wrote), _addr(lengths), _addr(counts) if counts is not None else 0, k.addr, v.addr,
                    n, c.heads, c.d, c.blocks, extra)
         return k, v
 

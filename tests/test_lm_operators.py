@@ -932,6 +932,36 @@ def test_cache_runtime_refuses_to_advance_by_what_does_not_fit():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("T", [40, 150])
+def test_cache_attends_to_what_was_written(T):
+    """Counts that only write() was given, more queries than rows, none written at all: what is there is attended to and read, the rest is zeros."""
+    require_gpu()
+    if hip.COMPILE_ONLY:
+        return
+    rng = np.random.default_rng(46)
+    B, d, n = 4, 32, np.array([T, 30, 0, 1])
+    k, v = rows_of(rng, B, T, d)
+    q = rng.standard_normal((B, T, d)).astype(f32)
+    cache, c = nn.QuantizedKVCache(B, 192, 1, d), hip_tensor(n.reshape(B, 1))
+    assert (cache.attend(hip_tensor(q)).numpy() == 0).all() and (cache.read(T, new=T)[0].numpy() == 0).all()
+    cache.write(hip_tensor(k), hip_tensor(v), counts=c)
+    want = cache.attend(hip_tensor(q), counts=c).numpy()
+    same(cache.attend(hip_tensor(q)).numpy(), want)
+    for b in range(B):
+        assert np.isfinite(want[b]).all() and (want[b, n[b]:] == 0).all()
+        if n[b]:
+            y, tol = attended(q[b, :n[b]].reshape(n[b], 1, d), *(held(a[b, :n[b]].reshape(n[b], 1, d), n[b] // 64 * 64) for a in (k, v)), 0, d ** -0.5, 1)
+            within(want[b, :n[b]].reshape(y.shape), y, tol, f"sequence {b}")
+    for a, z, w in zip(cache.read(T, new=T), cache.read(T, counts=c), (k, v)):
+        same(a.numpy(), z.numpy())
+        for b in range(B):
+            same(a.numpy()[b, :n[b]], held(w[b, :n[b]].reshape(n[b], 1, d), n[b] // 64 * 64).reshape(n[b], d))
+    cache.advance(c)
+    assert (cache.attend(hip_tensor(q)).numpy() == 0).all()
+    same(cache.read(192, new=5)[0].numpy(), cache.read(192)[0].numpy())
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("seed", range(6))
 def test_cache_gives_its_own_tokens_or_nan(seed):
     """Writes of any length, replaced and advanced over by any part of them: every position reads as its token, or as NaN in a block that
